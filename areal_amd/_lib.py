@@ -66,6 +66,19 @@ SIGNATURES: dict[str, tuple] = {
         I,
         [P, I, I64, P, I64, I64, F, P, P, P, P, P, I64, P],
     ),
+    "areal_sample_tokens_workspace_bytes": (SZ, [I64, I64]),
+    "areal_sample_tokens": (
+        I,
+        [P, I, I64, I64, I64, P, I, D, P, I64, P, I, D, P, D, P, P, P, P, P, I64, P, SZ, P],
+    ),
+    "areal_kept_logprobs_entropy_fwd": (I, [P, I, I64, P, P, I64, I64, I64, F, P, P, P, P]),
+    "areal_kept_logprobs_entropy_bwd": (
+        I,
+        [P, I, I64, P, P, I64, I64, I64, F, P, P, P, P, P, I64, P],
+    ),
+    "areal_embedding_fwd": (I, [P, I, I64, P, I64, I64, I64, F, P, I, P]),
+    "areal_embedding_bwd_workspace_bytes": (SZ, [I64, I64, I64]),
+    "areal_embedding_bwd": (I, [P, I, P, I64, I64, I64, F, I64, P, I, I, P, SZ, P]),
     "areal_actor_loss_workspace_bytes": (SZ, [I64, I64]),
     "areal_actor_loss": (
         I,

@@ -870,6 +870,181 @@ variable_list logits_logprobs(const Tensor& logits, const Tensor& labels, double
 }
 
 // ---------------------------------------------------------------------------------------
+// Next tokens, and log-probabilities under the sets they were drawn from
+// ---------------------------------------------------------------------------------------
+int dtype_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
+
+// [N, V] with a unit stride and rows that do not overlap, in a type the kernels read.
+Tensor logit_rows(const Tensor& logits) {
+  Tensor rows = logits.requires_grad() ? logits.detach() : logits;
+  if (dtype_code(rows.scalar_type()) < 0) rows = rows.to(at::kFloat);
+  const int64_t V = rows.size(-1);
+  if (rows.dim() != 2) rows = rows.reshape({rows.numel() / V, V});
+  if ((V > 1 && rows.stride(-1) != 1) || (rows.size(0) > 1 && rows.stride(0) < V)) rows = rows.contiguous();
+  return rows;
+}
+int64_t pitch_of(const Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+// One value per row (a tensor), or one for all.
+struct RowSetting {
+  Tensor rows;
+  RowSetting(const OptTensor& t, int64_t n, const char* name, bool whole) {
+    if (!t.has_value()) return;
+    require_numel(n, {{name, &*t}});
+    const at::ScalarType type = !whole ? at::kFloat : t->scalar_type() == at::kInt ? at::kInt : at::kLong;
+    rows = flat(*t, type);
+  }
+};
+
+py::tuple sample_tokens(const Tensor& logits, const Tensor& uniforms, const OptTensor& temperature_rows,
+                        double temperature, const OptTensor& top_k_rows, int64_t top_k, const OptTensor& top_p_rows,
+                        double top_p, const OptTensor& min_p_rows, double min_p, bool with_kept) {
+  refuse_tangent(logits);
+  require_gpu(logits, uniforms, or_undefined(temperature_rows), or_undefined(top_k_rows), or_undefined(top_p_rows),
+              or_undefined(min_p_rows));
+  const c10::hip::HIPGuard guard(logits.device().index());
+  const Tensor rows = logit_rows(logits);
+  const int64_t N = rows.size(0), V = rows.size(1), words = (V + 31) / 32;
+  require_numel(N, {{"uniforms", &uniforms}});
+  const Tensor u = flat(uniforms, uniforms.scalar_type());
+  const RowSetting tau(temperature_rows, N, "temperature", false), k(top_k_rows, N, "top_k", true),
+      p(top_p_rows, N, "top_p", false), least(min_p_rows, N, "min_p", false);
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const Tensor tokens = empty(rows, lead, at::kLong), lp = empty(rows, lead, at::kFloat),
+               full = empty(rows, lead, at::kFloat);
+  Tensor kept;
+  if (with_kept) {
+    auto shape = lead.vec();
+    shape.push_back(words);
+    kept = empty(rows, shape, at::kInt);
+  }
+  const size_t bytes = areal_sample_tokens_workspace_bytes(N, V);
+  const Tensor ws = workspace(rows, bytes);
+  check(areal_sample_tokens(ptr<void>(rows), dtype_code(rows.scalar_type()), pitch_of(rows), N, V, ptr<void>(u),
+                            u.scalar_type() == at::kDouble, temperature, ptr<float>(tau.rows), top_k,
+                            ptr<void>(k.rows), k.rows.defined() && k.rows.scalar_type() == at::kLong, top_p,
+                            ptr<float>(p.rows), min_p, ptr<float>(least.rows), ptr<int64_t>(tokens), ptr<float>(lp),
+                            ptr<float>(full), ptr<uint32_t>(kept), words, ptr<void>(ws), bytes, stream_of(rows)),
+        "areal_sample_tokens");
+  return py::make_tuple(tokens, lp, full, kept.defined() ? py::cast(kept) : py::none());
+}
+
+struct KeptLogits : public torch::autograd::Function<KeptLogits> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& kept,
+                               double temperature, bool needs_grad) {
+    const Tensor rows = logit_rows(logits);
+    const int64_t N = rows.size(0), V = rows.size(1);
+    const Tensor lab = flat(labels, at::kLong);
+    const Tensor words = kept.reshape({N, kept.size(-1)}).contiguous();
+    const Tensor lp = empty(rows, labels.sizes(), at::kFloat), ent = empty(rows, labels.sizes(), at::kFloat);
+    const Tensor lse2 = needs_grad ? empty_f32(rows, N) : Tensor();
+    check(areal_kept_logprobs_entropy_fwd(ptr<void>(rows), dtype_code(rows.scalar_type()), pitch_of(rows),
+                                          ptr<int64_t>(lab), ptr<uint32_t>(words), words.size(1), N, V,
+                                          (float)(1.0 / temperature), ptr<float>(lp), ptr<float>(ent),
+                                          ptr<float>(lse2), stream_of(rows)),
+          "areal_kept_logprobs_entropy_fwd");
+    ctx->save_for_backward({rows, lab, words, lse2, ent});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["shape"] = logits.sizes().vec();
+    ctx->saved_data["type"] = (int64_t)logits.scalar_type();
+    ctx->set_materialize_grads(false);
+    return {lp, ent};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(5);
+    if (!grads[0].defined() && !grads[1].defined()) return r;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &rows = saved[0], &lab = saved[1], &words = saved[2], &lse2 = saved[3], &ent = saved[4];
+    const c10::hip::HIPGuard guard(rows.device().index());
+    const int64_t N = rows.size(0), V = rows.size(1);
+    const Tensor glp = flat(grads[0], at::kFloat), gen = flat(grads[1], at::kFloat);
+    Tensor d = empty(rows, {N, V}, rows.scalar_type());
+    check(areal_kept_logprobs_entropy_bwd(ptr<void>(rows), dtype_code(rows.scalar_type()), pitch_of(rows),
+                                          ptr<int64_t>(lab), ptr<uint32_t>(words), words.size(1), N, V,
+                                          (float)(1.0 / ctx->saved_data["temperature"].toDouble()), ptr<float>(lse2),
+                                          ptr<float>(ent), ptr<float>(glp), ptr<float>(gen), ptr<void>(d), V,
+                                          stream_of(rows)),
+          "areal_kept_logprobs_entropy_bwd");
+    d = d.view(ctx->saved_data["shape"].toIntVector());
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    r[0] = d.scalar_type() == type ? d : d.to(type);
+    return r;
+  }
+};
+
+variable_list kept_logprobs(const Tensor& logits, const Tensor& labels, const Tensor& kept, double temperature) {
+  refuse_tangent(logits);
+  require_gpu(logits, labels, kept);
+  const c10::hip::HIPGuard guard(logits.device().index());
+  return KeptLogits::apply(logits, labels, kept, temperature, wants_grad(logits));
+}
+
+// ---------------------------------------------------------------------------------------
+// Embedding lookup
+// ---------------------------------------------------------------------------------------
+struct Accumulator {  // (not a tensor: no input of the node)
+  Tensor into;
+};
+
+struct Embedding : public torch::autograd::Function<Embedding> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale,
+                               int64_t padding_idx, at::ScalarType out_type, const Accumulator& accum) {
+    const int64_t V = weight.size(0), H = weight.size(1);
+    Tensor w = weight.requires_grad() ? weight.detach() : weight;
+    if ((H > 1 && w.stride(1) != 1) || (V > 1 && w.stride(0) < H)) w = w.contiguous();
+    const Tensor id = flat(ids, at::kLong);
+    const int64_t T = id.numel();
+    auto shape = ids.sizes().vec();
+    shape.push_back(H);
+    const Tensor out = empty(w, shape, out_type);
+    check(areal_embedding_fwd(ptr<void>(w), dtype_code(w.scalar_type()), pitch_of(w), ptr<int64_t>(id), T, H, V,
+                              (float)scale, ptr<void>(out), dtype_code(out_type), stream_of(w)),
+          "areal_embedding_fwd");
+    ctx->save_for_backward({id});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_idx"] = padding_idx;
+    ctx->saved_data["V"] = V;
+    ctx->saved_data["H"] = H;
+    ctx->saved_data["type"] = (int64_t)w.scalar_type();
+    if (accum.into.defined()) ctx->saved_data["accum"] = accum.into;
+    ctx->set_materialize_grads(false);
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(6);
+    if (!grads[0].defined()) return r;
+    const Tensor id = ctx->get_saved_variables()[0];
+    const c10::hip::HIPGuard guard(id.device().index());
+    const int64_t V = ctx->saved_data["V"].toInt(), H = ctx->saved_data["H"].toInt(), T = id.numel();
+    const Tensor g = grads[0].contiguous();
+    const auto found = ctx->saved_data.find("accum");
+    const bool add = found != ctx->saved_data.end();
+    const Tensor dw = add ? found->second.toTensor()
+                          : empty(g, {V, H}, (at::ScalarType)ctx->saved_data["type"].toInt());
+    const size_t bytes = areal_embedding_bwd_workspace_bytes(T, H, V);
+    const Tensor ws = workspace(g, bytes);
+    check(areal_embedding_bwd(ptr<void>(g), dtype_code(g.scalar_type()), ptr<int64_t>(id), T, H, V,
+                              (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding_idx"].toInt(),
+                              ptr<void>(dw), dtype_code(dw.scalar_type()), add ? 1 : 0, ptr<void>(ws), bytes,
+                              stream_of(g)),
+          "areal_embedding_bwd");
+    if (!add) r[0] = dw;
+    return r;
+  }
+};
+
+Tensor embed_tokens(const Tensor& ids, const Tensor& weight, double scale, int64_t padding_idx,
+                    const py::object& out_type, const OptTensor& accum) {
+  refuse_tangent(weight);
+  const Accumulator into{or_undefined(accum)};
+  require_gpu(ids, weight, into.into);
+  const c10::hip::HIPGuard guard(weight.device().index());
+  const at::ScalarType type =
+      out_type.is_none() ? weight.scalar_type() : torch::python::detail::py_object_to_dtype(out_type);
+  return Embedding::apply(weight, ids, scale, padding_idx, type, into)[0];
+}
+
+// ---------------------------------------------------------------------------------------
 // Advantages
 // ---------------------------------------------------------------------------------------
 // What a group normalisation needs besides its data: (group offsets [G + 1], rows per group [G], longest
@@ -1426,6 +1601,9 @@ PYBIND11_MODULE(_host, m) {
   m.def("lm_head_backward", &lm_head_backward);
   m.def("default_token_chunk", &default_token_chunk);
   m.def("logits_logprobs", &logits_logprobs);
+  m.def("sample_tokens", &sample_tokens);
+  m.def("kept_logprobs", &kept_logprobs);
+  m.def("embed_tokens", &embed_tokens);
   py::class_<HostInt>(m, "HostInt").def("wait", &HostInt::wait);
   m.def("advantage_prep", &advantage_prep);
   m.def("gae_row_stats", &gae_row_stats);

@@ -33,6 +33,10 @@ template <> struct Elem<float> {
     f32x4 v = {o[0], o[1], o[2], o[3]};
     __builtin_nontemporal_store(v, (f32x4*)p);
   }
+  static DEVI void storeu(float* p, const float* o) {  // from any element
+    const f32x4 v = {o[0], o[1], o[2], o[3]};
+    __builtin_nontemporal_store(v, (Vec*)p);
+  }
 };
 template <> struct Elem<u16> {  // bf16 bit patterns
   typedef u32x4 Vec __attribute__((aligned(2)));
@@ -52,6 +56,30 @@ template <> struct Elem<u16> {  // bf16 bit patterns
     for (int i = 0; i < 4; ++i)
       v[i] = (uint32_t)f32_to_bf16_bits(o[2 * i]) | ((uint32_t)f32_to_bf16_bits(o[2 * i + 1]) << 16);
     __builtin_nontemporal_store(v, (u32x4*)p);
+  }
+  static DEVI void storeu(u16* p, const float* o) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack_bf16x2(o[2 * i], o[2 * i + 1]);
+    __builtin_nontemporal_store(v, (Vec*)p);
+  }
+};
+
+template <> struct Elem<_Float16> {
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  typedef f16x8 Vec __attribute__((aligned(2)));
+  static constexpr int VEC = 8;
+  static DEVI float load(const _Float16* p) { return (float)*p; }
+  static DEVI void widen(const f16x8& v, float* o) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)v[i];
+  }
+  static DEVI void store(_Float16* p, float v) { *p = (_Float16)v; }
+  static DEVI void storeu(_Float16* p, const float* o) {
+    f16x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (_Float16)o[i];
+    __builtin_nontemporal_store(v, (Vec*)p);
   }
 };
 
@@ -313,6 +341,229 @@ int launch_rows_bwd(const void* logits, int64_t ld, const int64_t* labels, int64
   return AREAL_OK;
 }
 
+// ---- over kept sets: the same with the softmax over the tokens whose bit is set ----
+// Bit j of word w of a row stands for token 32 w + j. A wave takes 2048 tokens at a time: a word per lane, and where
+// one is not empty each lane the logits of four of their bytes, 512 tokens in one step. Logits without a bit are not
+// looked at (8 neighbours without one not even read), so a row that keeps few costs its bits.
+constexpr int64_t KEPT_MAX_ROWS = BWD_MAX_BLOCKS / 2;  // a block of up to 1024 threads each
+constexpr int KEPT_STEP = 2048, KEPT_UNIT = 8, KEPT_STEPS = 4;
+// Exponents are held above this: a kept logit of -inf then adds 0 to sums of t * 2^t (a NaN stays one).
+constexpr float KEPT_LOWEST = -160.f;
+
+template <typename T>
+DEVI void load_unit(const T* x, int at, int V, float (&z)[KEPT_UNIT]) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (at + KEPT_UNIT <= V) {
+    typename Elem<T>::Vec v[KEPT_UNIT / VEC];
+#pragma unroll
+    for (int i = 0; i < KEPT_UNIT / VEC; ++i) v[i] = *(const typename Elem<T>::Vec*)(x + at + i * VEC);
+#pragma unroll
+    for (int i = 0; i < KEPT_UNIT / VEC; ++i) Elem<T>::widen(v[i], z + i * VEC);
+  } else {
+#pragma unroll
+    for (int i = 0; i < KEPT_UNIT; ++i) z[i] = at + i < V ? Elem<T>::load(x + at + i) : neg_inf();
+  }
+}
+// Word `w` of a row; bits behind the vocabulary do not count.
+DEVI uint32_t kept_word(const uint32_t* kept, int w, int V) {
+  if (w * 32 >= V) return 0;
+  const uint32_t bits = kept[w];
+  return V - w * 32 >= 32 ? bits : bits & ((1u << (V - w * 32)) - 1);
+}
+// Byte of unit `step * 64 + lane` of the wave's 256, out of the lanes' words.
+DEVI uint32_t kept_byte(uint32_t word, int step, int lane) {
+  return (__shfl((int)word, step * 16 + (lane >> 2), 64) >> ((lane & 3) * 8)) & 0xff;
+}
+DEVI bool kept_at(const uint32_t* kept, int64_t token) { return kept[token >> 5] >> (token & 31) & 1; }
+
+DEVI void online_add_kept(Online& st, const float (&x)[KEPT_UNIT], uint32_t bits, float c2) {
+  float z[KEPT_UNIT], xm = neg_inf();
+#pragma unroll
+  for (int i = 0; i < KEPT_UNIT; ++i) {
+    z[i] = bits >> i & 1 ? x[i] : neg_inf();
+    xm = fmaxf(xm, z[i]);
+  }
+  const float vm = xm * c2;
+  if (vm > st.m) {
+    if (st.m > neg_inf()) {
+      const float d = st.m - vm, al = fast_exp2(d);
+      st.q = al * fmaf(d, st.s, st.q);
+      st.s = al * st.s;
+    }
+    st.m = vm;
+  }
+  const float m = st.m > neg_inf() ? st.m : 0.f;
+#pragma unroll
+  for (int i = 0; i < KEPT_UNIT; ++i) {
+    const float t = stat_max(fmaf(z[i], c2, -m), KEPT_LOWEST);
+    const float e = fast_exp2(t);
+    st.s += e;
+    st.q = fmaf(t, e, st.q);
+  }
+}
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__ logits, int64_t ld,
+                                                           const int64_t* __restrict__ labels,
+                                                           const uint32_t* __restrict__ kept, int64_t kept_ld, int V,
+                                                           float inv_temp, float* __restrict__ logprobs,
+                                                           float* __restrict__ entropy, float* __restrict__ lse2_out) {
+  __shared__ Online smem[THREADS / 64];
+  constexpr int WAVES = THREADS / 64, AHEAD = 4;
+  const int64_t row = blockIdx.x;
+  const T* const x = logits + row * ld;
+  const uint32_t* const bits = kept + row * kept_ld;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float c2 = inv_temp * LOG2E_F;
+  Online st{neg_inf(), 0.f, 0.f};
+  for (int64_t c0 = (int64_t)wave * KEPT_STEP; c0 < V; c0 += (int64_t)AHEAD * WAVES * KEPT_STEP) {
+    uint32_t words[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int64_t c = c0 + (int64_t)a * WAVES * KEPT_STEP;
+      words[a] = c < V ? kept_word(bits, (int)(c / 32) + lane, V) : 0;
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (__builtin_amdgcn_ballot_w64(words[a] != 0) == 0) continue;
+      const int c = (int)(c0 + (int64_t)a * WAVES * KEPT_STEP);
+      float z[KEPT_STEPS][KEPT_UNIT];
+      uint32_t b[KEPT_STEPS];
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i) {
+        b[i] = kept_byte(words[a], i, lane);
+        if (b[i] != 0) load_unit<T>(x, c + (i * 64 + lane) * KEPT_UNIT, V, z[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i)
+        if (b[i] != 0) online_add_kept(st, z[i], b[i], c2);
+    }
+  }
+  const Online r = block_merge(st, smem);
+  if (threadIdx.x == 0) {
+    const float log2s = fast_log2(r.s);
+    const bool none = r.m == neg_inf() && r.s == 0.f;  // no kept logit above -inf
+    const int64_t lab = labels[row];
+    float lp = 0.f;
+    if (r.s != r.s) {
+      lp = r.s;
+    } else if (lab >= 0 && lab < V) {
+      lp = neg_inf();
+      if (!none && kept_at(bits, lab)) {
+        lp = (fmaf(Elem<T>::load(x + lab), c2, -r.m) - log2s) * LN2_F;
+        lp = lp > 0.f ? 0.f : lp;
+      }
+    }
+    logprobs[row] = lp;
+    if (entropy) entropy[row] = none ? 0.f : (log2s - r.q / r.s) * LN2_F;
+    if (lse2_out) lse2_out[row] = none ? pos_inf() : r.m + log2s;  // +inf: every probability is 0
+  }
+}
+
+// Block (row, part): part_steps runs of KEPT_STEP tokens.
+constexpr int KEPT_BWD_WAVES = 4;
+template <typename T, bool ENT>
+__global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
+    const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, const uint32_t* __restrict__ kept,
+    int64_t kept_ld, int V, float inv_temp, const float* __restrict__ lse2, const float* __restrict__ entropy,
+    const float* __restrict__ grad_lp, const float* __restrict__ grad_ent, T* __restrict__ dlogits, int64_t ldd,
+    unsigned parts, unsigned part_steps) {
+  constexpr int VEC = Elem<T>::VEC;
+  const int64_t row = blockIdx.x / parts;
+  const unsigned part = blockIdx.x % parts;
+  const T* const x = logits + row * ld;
+  T* const d = dlogits + row * ldd;
+  const uint32_t* const bits = kept + row * kept_ld;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float c2 = inv_temp * LOG2E_F;
+  const float l2 = lse2[row];
+  const int64_t lab64 = labels[row];
+  // a label outside the kept set has log-probability -inf, whose gradient is taken as 0
+  const bool labelled = lab64 >= 0 && lab64 < V && kept_at(bits, lab64) && !(Elem<T>::load(x + lab64) == neg_inf());
+  const int lab = labelled ? (int)lab64 : -1;
+  const float glp = labelled && grad_lp ? grad_lp[row] * inv_temp : 0.f;
+  const float gen = ENT ? grad_ent[row] * inv_temp : 0.f;
+  const float ent = ENT ? entropy[row] : 0.f;
+  const bool none = l2 == pos_inf();
+  for (unsigned step = wave; step < part_steps; step += KEPT_BWD_WAVES) {
+    const int64_t c64 = ((int64_t)part * part_steps + step) * KEPT_STEP;
+    if (c64 >= V) return;
+    const int c = (int)c64;
+    const uint32_t word = none ? 0 : kept_word(bits, c / 32 + lane, V);
+    float z[KEPT_STEPS][KEPT_UNIT];
+    uint32_t b[KEPT_STEPS];
+#pragma unroll
+    for (int i = 0; i < KEPT_STEPS; ++i) {
+      b[i] = kept_byte(word, i, lane);
+      if (b[i] != 0) load_unit<T>(x, c + (i * 64 + lane) * KEPT_UNIT, V, z[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < KEPT_STEPS; ++i) {
+      const int at = c + (i * 64 + lane) * KEPT_UNIT;
+      if (at >= V) continue;
+      float g[KEPT_UNIT];
+#pragma unroll
+      for (int j = 0; j < KEPT_UNIT; ++j) g[j] = 0.f;
+      if (b[i] != 0) {
+#pragma unroll
+        for (int j = 0; j < KEPT_UNIT; ++j) {
+          const float t = stat_max(fmaf(z[i][j], c2, -l2), KEPT_LOWEST);
+          const float p = fast_exp2(t);
+          float v = -p * glp;
+          if (at + j == lab) v += glp;
+          if (ENT) v -= gen * p * (t * LN2_F + ent);
+          g[j] = b[i] >> j & 1 ? v : 0.f;
+        }
+      }
+      if (at + KEPT_UNIT <= V) {
+#pragma unroll
+        for (int j = 0; j < KEPT_UNIT / VEC; ++j) Elem<T>::storeu(d + at + j * VEC, g + j * VEC);
+      } else {
+#pragma unroll
+        for (int j = 0; j < KEPT_UNIT; ++j)
+          if (at + j < V) Elem<T>::store(d + at + j, g[j]);
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_kept_fwd(const void* logits, int64_t ld, const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
+                    int64_t N, int64_t V, float inv_temp, float* lp, float* ent, float* lse2, hipStream_t stream) {
+  auto launch = [&](auto threads) {
+    constexpr int THREADS = decltype(threads)::value;
+    hipLaunchKernelGGL((kept_fwd_kernel<T, THREADS>), dim3((unsigned)N), dim3(THREADS), 0, stream, (const T*)logits, ld,
+                       labels, kept, kept_ld, (int)V, inv_temp, lp, ent, lse2);
+  };
+  if (N < FWD_FEW_ROWS)
+    launch(std::integral_constant<int, 1024>{});
+  else
+    launch(std::integral_constant<int, 256>{});
+  AREAL_CHECK_LAUNCH();
+  return AREAL_OK;
+}
+
+template <typename T>
+int launch_kept_bwd(const void* logits, int64_t ld, const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
+                    int64_t N, int64_t V, float inv_temp, const float* lse2, const float* ent, const float* glp,
+                    const float* gent, void* dlogits, int64_t ldd, hipStream_t stream) {
+  const int64_t steps = ceil_div_i64(V, KEPT_STEP);
+  int64_t parts = ceil_div_i64(steps, KEPT_BWD_WAVES);
+  parts = std::min(parts, std::max<int64_t>(BWD_MAX_BLOCKS / N, 1));
+  const int64_t part_steps = ceil_div_i64(steps, parts);
+  auto launch = [&](auto with_entropy) {
+    hipLaunchKernelGGL((kept_bwd_kernel<T, decltype(with_entropy)::value>), dim3((unsigned)(N * parts)),
+                       dim3(64 * KEPT_BWD_WAVES), 0, stream, (const T*)logits, ld, labels, kept, kept_ld, (int)V,
+                       inv_temp, lse2, ent, glp, gent, (T*)dlogits, ldd, (unsigned)parts, (unsigned)part_steps);
+  };
+  if (gent)
+    launch(std::true_type{});
+  else
+    launch(std::false_type{});
+  AREAL_CHECK_LAUNCH();
+  return AREAL_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -357,6 +608,38 @@ int areal_logits_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld,
     return launch_rows_bwd<u16>(logits, ld, labels, T, V, inv_temperature, lse2, entropy,
                                 grad_logprobs, grad_entropy, dlogits, ldd, stream);
   return AREAL_ERR_BAD_ARG;
+}
+
+// dtype: 0 = fp32, 1 = bf16, 2 = fp16. kept [N, kept_ld] words.
+int areal_kept_logprobs_entropy_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels,
+                                    const uint32_t* kept, int64_t kept_ld, int64_t N, int64_t V, float inv_temperature,
+                                    float* logprobs, float* entropy, float* lse2, hipStream_t stream) {
+  if (N < 0 || V <= 0 || ld < V || kept_ld < ceil_div_i64(V, 32) || !(inv_temperature > 0.f)) return AREAL_ERR_BAD_ARG;
+  if (N == 0) return AREAL_OK;
+  if (!logits || !labels || !kept || !logprobs) return AREAL_ERR_BAD_ARG;
+  if (V > (1 << 30) || N > KEPT_MAX_ROWS) return AREAL_ERR_UNSUPPORTED;
+  auto run = [&](auto t) {
+    return launch_kept_fwd<decltype(t)>(logits, ld, labels, kept, kept_ld, N, V, inv_temperature, logprobs, entropy,
+                                        lse2, stream);
+  };
+  return dtype == 0 ? run(float{}) : dtype == 1 ? run(u16{}) : dtype == 2 ? run(_Float16{}) : AREAL_ERR_BAD_ARG;
+}
+
+int areal_kept_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld, const int64_t* labels,
+                                    const uint32_t* kept, int64_t kept_ld, int64_t N, int64_t V, float inv_temperature,
+                                    const float* lse2, const float* entropy, const float* grad_logprobs,
+                                    const float* grad_entropy, void* dlogits, int64_t ldd, hipStream_t stream) {
+  if (N < 0 || V <= 0 || ld < V || ldd < V || kept_ld < ceil_div_i64(V, 32) || !(inv_temperature > 0.f))
+    return AREAL_ERR_BAD_ARG;
+  if (N == 0) return AREAL_OK;
+  if (!logits || !labels || !kept || !lse2 || !dlogits) return AREAL_ERR_BAD_ARG;
+  if (grad_entropy != nullptr && entropy == nullptr) return AREAL_ERR_BAD_ARG;
+  if (V > (1 << 30) || N > KEPT_MAX_ROWS) return AREAL_ERR_UNSUPPORTED;
+  auto run = [&](auto t) {
+    return launch_kept_bwd<decltype(t)>(logits, ld, labels, kept, kept_ld, N, V, inv_temperature, lse2, entropy,
+                                        grad_logprobs, grad_entropy, dlogits, ldd, stream);
+  };
+  return dtype == 0 ? run(float{}) : dtype == 1 ? run(u16{}) : dtype == 2 ? run(_Float16{}) : AREAL_ERR_BAD_ARG;
 }
 
 }  // extern "C"

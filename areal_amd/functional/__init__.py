@@ -16,10 +16,16 @@ from areal_amd.functional.aux_losses import (
     ppo_critic_loss_fn,
     sapo_loss_fn,
 )
+from areal_amd.functional.embedding import embed_tokens
 from areal_amd.functional.lm_head import (
     ChunkedLMHeadOutput,
     chunked_lm_head_logprobs_entropy,
     fused_lm_head_logprobs_entropy,
+)
+from areal_amd.functional.sampling import (
+    SampledTokens,
+    gather_kept_logprobs_entropy,
+    sample_tokens,
 )
 from areal_amd.functional.vocab_parallel import (
     gather_logprobs,
@@ -44,4 +50,8 @@ __all__ = [
     "ChunkedLMHeadOutput",
     "chunked_lm_head_logprobs_entropy",
     "fused_lm_head_logprobs_entropy",
+    "SampledTokens",
+    "sample_tokens",
+    "gather_kept_logprobs_entropy",
+    "embed_tokens",
 ]

@@ -1,0 +1,153 @@
+"""Next tokens from logits, and label log-probabilities under the sets they were drawn from: the
+rollout's and the trainer's side of one distribution.
+
+``sample_tokens`` returns the log-probability of each token in the truncated distribution it was
+drawn from and in the whole one; the latter is what ``gather_logprobs`` computes for it. With
+``return_kept`` it also returns the truncated sets, and ``gather_kept_logprobs_entropy`` computes
+log-probabilities (and their gradient) over those sets, so that the importance ratio of a token
+drawn with top-k, top-p or min-p is that of two distributions over the same tokens.
+
+The kernels are ``csrc/sampling.hip`` and the kept-set kernels of ``csrc/logits_rows.hip``.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from areal_amd import _lib
+
+MAX_VOCAB = 1 << 22  # of sample_tokens
+
+
+class SampledTokens(NamedTuple):
+    """``kept``: int32 ``[..., ceil(V / 32)]``, bit ``j`` of word ``w`` is token ``32 w + j``; ``None``
+    unless asked for."""
+
+    tokens: torch.Tensor
+    logprobs: torch.Tensor
+    full_logprobs: torch.Tensor
+    kept: torch.Tensor | None
+
+
+def _setting(name: str, value, default, low, high, whole: bool = False):
+    """(tensor or None, number) of a setting given as a number, a tensor with one value a row, or None."""
+    if value is None:
+        return None, default
+    if torch.is_tensor(value):
+        if whole and (value.is_floating_point() or value.is_complex() or value.dtype == torch.bool):
+            raise ValueError(f"{name} must be a tensor of integers, got {value.dtype}")
+        if not whole and not value.is_floating_point():
+            raise ValueError(f"{name} must be a floating-point tensor, got {value.dtype}")
+        return value, default
+    if whole and (isinstance(value, bool) or int(value) != value):
+        raise ValueError(f"{name} must be an integer, got {value}")
+    if not whole and not math.isfinite(value):
+        raise ValueError(f"{name} must be finite, got {value}")
+    if not low <= value <= high:
+        raise ValueError(f"{name} must lie in [{low}, {high}], got {value}")
+    return None, int(value) if whole else float(value)
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor | None = None,
+    top_p: float | torch.Tensor | None = None,
+    min_p: float | torch.Tensor | None = None,
+    return_kept: bool = False,
+) -> SampledTokens:
+    """One token per row of ``logits``, by inversion of its distribution at ``uniforms``.
+
+    With ``e_i = exp((x_i - max x) / temperature)`` and the logits in descending order (ties: the
+    lowest index first), ``S1`` are the first ``top_k``, ``S2`` the shortest prefix of ``S1`` with at
+    least ``top_p`` of its mass, and ``S3`` the logits of ``S2`` with ``e_i >= min_p``. The token is the
+    first of ``S3``, by index, whose running mass passes ``uniforms`` times that of ``S3``. Masses
+    are 64-bit, and a token does not depend on how many rows a call has.
+
+    Args:
+        logits: ``[..., V]``, fp32, bf16 or fp16 (other types are converted to fp32), ``V`` up to
+            ``MAX_VOCAB``; logits of ``-inf`` are never drawn.
+        uniforms: ``[...]`` fp32 or fp64 numbers in ``[0, 1)`` (others are clamped, a NaN counts as 0).
+        temperature: a number >= 0, or a tensor with one per row; 0 (or below, in a tensor) takes the
+            first of the largest logits, with log-probabilities 0.
+        top_k: a number, or an integer tensor; ``None``, 0 and below: no limit.
+        top_p: a number in (0, 1], or a tensor (1 and above: no limit, 0 and below: the first alone).
+        min_p: a number in [0, 1], or a tensor (clamped to that).
+        return_kept: also return ``S3`` as bits.
+
+    Returns:
+        ``SampledTokens``: int64 tokens and fp32 log-probabilities in ``S3`` and in the whole row. A row
+        with a NaN or ``+inf`` logit, without a finite one, or with a NaN setting gives token -1,
+        NaN log-probabilities and an empty set. None of the outputs has a gradient.
+    """
+    if logits.ndim == 0 or logits.size(-1) == 0:
+        raise ValueError(f"logits must have at least one element per row, got {tuple(logits.shape)}")
+    if logits.size(-1) > MAX_VOCAB:
+        raise ValueError(f"at most {MAX_VOCAB} logits a row are supported, got {logits.size(-1)}")
+    if not logits.is_floating_point():
+        raise ValueError(f"logits must be floating-point, got {logits.dtype}")
+    lead = tuple(logits.shape[:-1])
+    if tuple(uniforms.shape) != lead:
+        raise ValueError(
+            "uniforms must match the leading dimensions of logits: "
+            f"got {tuple(uniforms.shape)} and {tuple(logits.shape)}"
+        )
+    if uniforms.dtype not in (torch.float32, torch.float64):
+        raise ValueError(f"uniforms must be fp32 or fp64, got {uniforms.dtype}")
+    settings = (
+        _setting("temperature", temperature, 1.0, 0.0, math.inf),
+        _setting("top_k", top_k, 0, -(1 << 62), 1 << 62, whole=True),
+        _setting("top_p", top_p, 1.0, math.ulp(0.0), 1.0),
+        _setting("min_p", min_p, 0.0, 0.0, 1.0),
+    )
+    for name, (rows, _) in zip(("temperature", "top_k", "top_p", "min_p"), settings):
+        if rows is not None and tuple(rows.shape) != lead:
+            raise ValueError(f"{name} must have one value per row, {lead}, got {tuple(rows.shape)}")
+    return SampledTokens(
+        *_lib.host().sample_tokens(logits, uniforms, *[x for pair in settings for x in pair], return_kept)
+    )
+
+
+def gather_kept_logprobs_entropy(
+    logits: torch.Tensor,
+    labels: torch.Tensor,
+    kept: torch.Tensor,
+    temperature: float = 1.0,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Label log-probabilities and entropy of ``softmax(logits / temperature)`` over the kept tokens
+    of each row; both are differentiable in ``logits`` (tokens that are not kept get gradient 0).
+
+    Args:
+        logits: ``[..., V]``, fp32, bf16 or fp16 (other types are converted to fp32). What stands at tokens
+            that are not kept does not matter, NaN and infinities included.
+        labels: ``[...]`` integer labels.
+        kept: int32 ``[..., W]``, ``W >= ceil(V / 32)``, as ``sample_tokens`` returns it; words of -1 keep all.
+        temperature: softmax temperature (> 0).
+
+    A label that is not kept has log-probability ``-inf``, without a gradient (leave such tokens out
+    of the loss); a row that keeps nothing has entropy 0 as well. A label outside ``[0, V)`` (an ignored
+    position) gives 0.
+    """
+    if not math.isfinite(temperature) or temperature <= 0:
+        raise ValueError(f"temperature must be positive, got {temperature}")
+    if logits.ndim == 0 or logits.size(-1) == 0:
+        raise ValueError(f"logits must have at least one element per row, got {tuple(logits.shape)}")
+    if not logits.is_floating_point():
+        raise ValueError(f"logits must be floating-point, got {logits.dtype}")
+    if tuple(logits.shape[:-1]) != tuple(labels.shape):
+        raise ValueError(
+            "logits leading dimensions must match labels: "
+            f"got {tuple(logits.shape)} and {tuple(labels.shape)}"
+        )
+    words = (logits.size(-1) + 31) // 32
+    if kept.dtype != torch.int32:
+        raise ValueError(f"kept must be int32, got {kept.dtype}")
+    if tuple(kept.shape[:-1]) != tuple(labels.shape) or kept.ndim == 0 or kept.size(-1) < words:
+        raise ValueError(
+            f"kept must have {words} words for each label: got {tuple(kept.shape)} for {tuple(labels.shape)}"
+        )
+    return tuple(_lib.host().kept_logprobs(logits, labels, kept, temperature))

@@ -165,6 +165,75 @@ int areal_logits_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld,
                                       areal_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Next tokens from logits, and label log-probabilities under the sets they were drawn from (the softmax of
+ * areal/utils/functional/vocab_parallel.py:16-30 over a kept set)
+ * ------------------------------------------------------------------------------------- */
+
+/* Workspace of areal_sample_tokens (0 for sizes it refuses). */
+size_t areal_sample_tokens_workspace_bytes(int64_t N, int64_t V);
+
+/* logits [N, V], row pitch ld (elements); dtype 0 fp32, 1 bf16, 2 fp16. uniforms [N], fp32 or
+ * (uniforms_fp64) fp64, in [0, 1) (clamped to [0, 1], a NaN counts as 0). Each setting is a number,
+ * or one per row where its *_rows is not NULL (top_k_rows: int32, or int64 with top_k_int64).
+ *   e_i = exp((x_i - max x) / temperature); in the order of descending x, ties by ascending index:
+ *   S1 = the first top_k (no limit: 0 or below, or V and above),
+ *   S2 = the shortest prefix of S1 whose mass is at least top_p times that of S1 (>= 1: S1; <= 0: its first),
+ *   S3 = the logits of S2 with e_i >= min_p (taken as at most 1).
+ * tokens[r] (int64) = the first index of S3 whose running mass, by index, passes uniforms[r] times that of S3;
+ * logprobs[r] = its log-probability in S3, full_logprobs[r] = in the whole row. Logits of -inf are in
+ * no set. temperature <= 0: the first of the largest logits, both log-probabilities 0. A row with a NaN
+ * or +inf logit, without a finite one, or with a NaN setting: token -1, NaN, nothing kept.
+ * kept (NULL to skip) [N, kept_ld] words, kept_ld >= ceil(V / 32): bit j of word w = token 32 w + j in S3
+ * (bits behind V are cleared, words behind them left alone). V is at most 2^22, else
+ * AREAL_ERR_UNSUPPORTED. */
+int areal_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t N, int64_t V,
+                        const void* uniforms, int uniforms_fp64, double temperature,
+                        const float* temperature_rows, int64_t top_k, const void* top_k_rows,
+                        int top_k_int64, double top_p, const float* top_p_rows, double min_p,
+                        const float* min_p_rows, int64_t* tokens, float* logprobs,
+                        float* full_logprobs, uint32_t* kept, int64_t kept_ld, void* workspace,
+                        size_t workspace_bytes, areal_stream_t stream);
+
+/* Log-probabilities of labels [N] (int64) and entropy (NULL to skip) of the softmax over the logits
+ * whose bit is set in kept (as above; other logits are not looked at, whatever they hold). A label in
+ * [0, V) that is not kept, or whose logit is -inf: -inf. A row that keeps nothing above -inf: -inf
+ * and entropy 0. A label outside [0, V): 0. A kept NaN or +inf: NaN. lse2 (NULL to skip): what
+ * the backward needs besides the entropy. */
+int areal_kept_logprobs_entropy_fwd(const void* logits, int dtype, int64_t ld,
+                                    const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
+                                    int64_t N, int64_t V, float inv_temperature, float* logprobs,
+                                    float* entropy, float* lse2, areal_stream_t stream);
+
+/* dlogits [N, V] (the type of the logits, row pitch ldd): 0 where nothing is kept; the log-probability
+ * of a label that is not kept has no gradient. Either upstream gradient may be NULL. */
+int areal_kept_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld,
+                                    const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
+                                    int64_t N, int64_t V, float inv_temperature, const float* lse2,
+                                    const float* entropy, const float* grad_logprobs,
+                                    const float* grad_entropy, void* dlogits, int64_t ldd,
+                                    areal_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Embedding lookup and its gradient (dtypes: 0 fp32, 1 bf16, 2 fp16)
+ * ------------------------------------------------------------------------------------- */
+
+/* out [T, H] = scale * weight[ids[t]], computed in fp32 and rounded once; weight [V, H] with row pitch
+ * ldw. An id outside [0, V) gives zeros (a shard's rows of other shards' ids). */
+int areal_embedding_fwd(const void* weight, int weight_dtype, int64_t ldw, const int64_t* ids,
+                        int64_t T, int64_t H, int64_t V, float scale, void* out, int out_dtype,
+                        areal_stream_t stream);
+
+size_t areal_embedding_bwd_workspace_bytes(int64_t T, int64_t H, int64_t V);
+
+/* dweight [V, H] = scale * the sums of grad [T, H] over the tokens of each id, in fp32 and in an order that
+ * is the same in every run; ids outside [0, V) and padding_idx (negative: none) give nothing. accumulate:
+ * added to dweight (fp32 only), whose other rows are left alone; else those are cleared. */
+int areal_embedding_bwd(const void* grad, int grad_dtype, const int64_t* ids, int64_t T, int64_t H,
+                        int64_t V, float scale, int64_t padding_idx, void* dweight,
+                        int dweight_dtype, int accumulate, void* workspace, size_t workspace_bytes,
+                        areal_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * Actor loss: PPO / GRPO clip (optionally dual clip, optionally GSPO sequence-level ratio) or
  * CISPO, with rejection sampling (IcePop ratio bounds, KPop binary KL, k1/k2/k3)
  * replaces ppo_actor_loss_fn (areal/utils/functional/functional.py:452-596), cispo_loss_fn

@@ -1,0 +1,143 @@
+"""Oracle: next tokens from logits, log-probabilities over kept sets, embedding lookup (CPU, fp64,
+test-only).
+
+The softmax and its entropy follow ``areal/utils/functional/vocab_parallel.py:16-30``, restricted to
+the kept tokens. Pinned by closed forms, by brute force over a grid of uniform numbers, and by
+differences for the gradients (``tests/test_oracle_token_ends.py``).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+NAN = float("nan")
+
+
+def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, log-probability in the kept set, in the row, kept set) of one row, element by element."""
+    x = [float(v) for v in x]
+    V, nothing = len(x), [False] * len(x)
+    top = max(x, default=-math.inf) if not any(math.isnan(v) for v in x) else NAN
+    if not math.isfinite(top) or any(math.isnan(float(s)) for s in (temperature, top_p, min_p)):
+        return -1, NAN, NAN, nothing
+    order = sorted(range(V), key=lambda i: (-x[i], i))
+    if temperature <= 0:
+        kept = list(nothing)
+        kept[order[0]] = True
+        return order[0], 0.0, 0.0, kept
+    e = [math.exp((v - top) / temperature) for v in x]
+    k = top_k if 0 < top_k < V else V
+    s1 = order[:k]
+    z1 = math.fsum(e[i] for i in s1)
+    s2, mass = [], 0.0
+    for i in s1:
+        if s2 and top_p < 1 and mass >= top_p * z1:
+            break
+        s2.append(i)
+        mass += e[i]
+    s3 = [i for i in s2 if e[i] >= min(min_p, 1.0) and x[i] > -math.inf]
+    kept = list(nothing)
+    for i in s3:
+        kept[i] = True
+    z3 = math.fsum(e[i] for i in s3)
+    u = 0.0 if math.isnan(u) else min(max(u, 0.0), 1.0)
+    token, cum = None, 0.0
+    for i in sorted(s3):
+        if e[i] > 0:
+            token = i
+            cum += e[i]
+            if cum > u * z3:
+                break
+    exponent = (x[token] - top) / temperature
+    return token, exponent - math.log(z3), exponent - math.log(math.fsum(e)), kept
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Settings: numbers, or tensors with one per row."""
+    def of(setting, i):
+        return setting[i].item() if torch.is_tensor(setting) else setting
+
+    rows = [
+        sample_row(logits[i].double().tolist(), float(uniforms[i]), *[of(s, i) for s in (temperature, top_k, top_p, min_p)])
+        for i in range(logits.shape[0])
+    ]
+    if not rows:
+        empty = torch.zeros(0, dtype=torch.float64)
+        return empty.long(), empty, empty, torch.zeros(0, logits.shape[1], dtype=torch.bool)
+    tokens, lp, full, kept = zip(*rows)
+    return torch.tensor(tokens), torch.tensor(lp, dtype=torch.float64), torch.tensor(full, dtype=torch.float64), torch.tensor(kept)
+
+
+def pack_bits(mask):
+    """Bool ``[N, V]`` to int32 ``[N, ceil(V / 32)]``."""
+    n, v = mask.shape
+    words = (v + 31) // 32
+    m = torch.zeros(n, words * 32, dtype=torch.int64)
+    m[:, :v] = mask.long()
+    w = (m.view(n, words, 32) << torch.arange(32)).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
+
+
+def kept_logprobs_entropy(logits, labels, mask, temperature=1.0):
+    x = logits.double() / temperature
+    lp = torch.zeros(x.shape[0], dtype=torch.float64)
+    ent = torch.zeros_like(lp)
+    for i in range(x.shape[0]):
+        z, lab = x[i][mask[i]], int(labels[i])
+        inside = 0 <= lab < x.shape[1]
+        if torch.isnan(z).any() or (z == math.inf).any():
+            lp[i] = ent[i] = NAN
+            continue
+        if z.numel() == 0 or z.max() == -math.inf:
+            lp[i] = -math.inf if inside else 0.0
+            continue
+        logp = z - torch.logsumexp(z, 0)
+        p = logp.exp()
+        ent[i] = -(p * logp)[p > 0].sum()
+        if inside:
+            lp[i] = x[i, lab] - torch.logsumexp(z, 0) if mask[i, lab] else -math.inf
+    return lp, ent
+
+
+def kept_backward(logits, labels, mask, grad_lp, grad_ent, temperature=1.0):
+    x = logits.double() / temperature
+    d = torch.zeros_like(x)
+    for i in range(x.shape[0]):
+        keep = mask[i] & (x[i] > -math.inf) | (mask[i] & torch.isnan(x[i]))
+        if not keep.any():
+            continue
+        z, lab = x[i][keep], int(labels[i])
+        if torch.isnan(z).any() or (z == math.inf).any():
+            d[i][keep] = NAN
+            continue
+        logp = z - torch.logsumexp(z, 0)
+        p = logp.exp()
+        h = -(p * logp).sum()
+        row = torch.zeros_like(z)
+        if 0 <= lab < x.shape[1] and keep[lab]:
+            one = (torch.nonzero(keep).view(-1) == lab).double()
+            row += float(grad_lp[i]) * (one - p)
+        row -= float(grad_ent[i]) * p * (logp + h)
+        d[i][keep] = row / temperature
+    return d
+
+
+def embedding(weight, ids, scale=1.0):
+    out = torch.zeros(*ids.shape, weight.shape[1], dtype=torch.float64)
+    inside = (ids >= 0) & (ids < weight.shape[0])
+    out[inside] = weight.double()[ids[inside]] * scale
+    return out
+
+
+def embedding_backward(grad, ids, shape, scale=1.0, padding_idx=None):
+    """(gradient, number of tokens and sum of |gradient| of each entry)."""
+    g, flat = grad.double().reshape(-1, shape[1]), ids.reshape(-1)
+    inside = (flat >= 0) & (flat < shape[0])
+    if padding_idx is not None:
+        inside &= flat != padding_idx
+    dw = torch.zeros(shape, dtype=torch.float64).index_add_(0, flat[inside], g[inside]) * scale
+    size = torch.zeros(shape, dtype=torch.float64).index_add_(0, flat[inside], g[inside].abs()) * abs(scale)
+    count = torch.bincount(flat[inside], minlength=shape[0])
+    return dw, count, size

@@ -1,0 +1,131 @@
+"""What sample_tokens, gather_kept_logprobs_entropy and embed_tokens refuse, in Python and at the C entry points.
+Needs no GPU: everything here is refused before a launch."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+from areal_amd import _lib
+from areal_amd.functional import embed_tokens, gather_kept_logprobs_entropy, sample_tokens
+
+X, U, Y = torch.zeros(3, 40), torch.zeros(3), torch.zeros(3, dtype=torch.long)
+K = torch.zeros(3, 2, dtype=torch.int32)
+W, I = torch.zeros(6, 8), torch.zeros(4, dtype=torch.long)
+
+
+@pytest.mark.parametrize("call, match", [
+    (lambda: sample_tokens(torch.zeros(3, 0), U), "at least one element"),
+    (lambda: sample_tokens(torch.zeros(()), torch.zeros(())), "at least one element"),
+    (lambda: sample_tokens(torch.zeros(1, (1 << 22) + 1, dtype=torch.bfloat16), U[:1]), "at most"),
+    (lambda: sample_tokens(X.long(), U), "floating-point"),
+    (lambda: sample_tokens(X, U[:2]), "uniforms must match"),
+    (lambda: sample_tokens(X, U.view(3, 1)), "uniforms must match"),
+    (lambda: sample_tokens(X, U.half()), "fp32 or fp64"),
+    (lambda: sample_tokens(X, U, temperature=-1.0), "temperature must lie"),
+    (lambda: sample_tokens(X, U, temperature=math.inf), "temperature must be finite"),
+    (lambda: sample_tokens(X, U, temperature=math.nan), "temperature must be finite"),
+    (lambda: sample_tokens(X, U, temperature=torch.ones(2)), "temperature must have one value per row"),
+    (lambda: sample_tokens(X, U, temperature=torch.ones(3, dtype=torch.int32)), "floating-point tensor"),
+    (lambda: sample_tokens(X, U, top_k=1.5), "top_k must be an integer"),
+    (lambda: sample_tokens(X, U, top_k=True), "top_k must be an integer"),
+    (lambda: sample_tokens(X, U, top_k=U), "tensor of integers"),
+    (lambda: sample_tokens(X, U, top_k=U > 0), "tensor of integers"),
+    (lambda: sample_tokens(X, U, top_p=0.0), "top_p must lie"),
+    (lambda: sample_tokens(X, U, top_p=1.1), "top_p must lie"),
+    (lambda: sample_tokens(X, U, min_p=-0.1), "min_p must lie"),
+    (lambda: sample_tokens(X, U, min_p=torch.zeros(3, 1)), "min_p must have one value per row"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K, 0.0), "temperature must be positive"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K, math.nan), "temperature must be positive"),
+    (lambda: gather_kept_logprobs_entropy(X, Y[:2], K), "must match labels"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K.long()), "kept must be int32"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K[:, :1]), "2 words for each label"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K[:2]), "2 words for each label"),
+    (lambda: gather_kept_logprobs_entropy(X.int(), Y, K), "floating-point"),
+    (lambda: gather_kept_logprobs_entropy(X[:, :0], Y, K), "at least one element"),
+    (lambda: embed_tokens(I, W[0]), r"weight must be \[V, H\]"),
+    (lambda: embed_tokens(I, W[:0]), r"weight must be \[V, H\]"),
+    (lambda: embed_tokens(I, W.double()), "weight must be fp32"),
+    (lambda: embed_tokens(I, W, out_dtype=torch.float64), "out_dtype must be fp32"),
+    (lambda: embed_tokens(I.float(), W), "input_ids must be integers"),
+    (lambda: embed_tokens(I > 0, W), "input_ids must be integers"),
+    (lambda: embed_tokens(I, W, math.inf), "scale must be finite"),
+    (lambda: embed_tokens(I, W, padding_idx=6), "padding_idx must lie"),
+    (lambda: embed_tokens(I, W, padding_idx=-1), "padding_idx must lie"),
+    (lambda: embed_tokens(I, W, weight_grad_accum=W.bfloat16()), "weight_grad_accum must be an fp32"),
+    (lambda: embed_tokens(I, W, weight_grad_accum=W[:5]), "weight_grad_accum must be an fp32"),
+    (lambda: embed_tokens(I, W, weight_grad_accum=torch.zeros(8, 6).t()), "must be contiguous"),
+    (lambda: embed_tokens(I, W, weight_grad_accum=torch.zeros(6, 8)), "requires a gradient"),
+])
+def test_values(call, match):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: sample_tokens(X, U),
+    lambda: gather_kept_logprobs_entropy(X, Y, K),
+    lambda: embed_tokens(I, W),
+])
+def test_no_cpu_fallback(call):
+    with pytest.raises(_lib.ArealHipError, match="no CPU fallback"):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: sample_tokens(x, U),
+    lambda x: gather_kept_logprobs_entropy(x, Y, K),
+    lambda x: embed_tokens(I, x),
+])
+def test_tangents(call):
+    with fwad.dual_level(), pytest.raises(NotImplementedError):
+        call(fwad.make_dual(X, torch.ones_like(X)))
+
+
+def test_c_entries_refuse_before_a_launch():
+    """No pointer here is one of a device: a launch would not go unnoticed."""
+    lib, p, null = _lib.load(), ctypes.c_void_p(4096), ctypes.c_void_p(0)
+
+    def sample(logits=p, dtype=1, ld=40, N=3, V=40, u=p, tau=1.0, tau_rows=null, top_p=1.0, min_p=0.0, tokens=p,
+               kept=null, kept_ld=2, ws=p, nbytes=None):
+        nbytes = lib.areal_sample_tokens_workspace_bytes(N, V) if nbytes is None else nbytes
+        return lib.areal_sample_tokens(logits, dtype, ld, N, V, u, 0, tau, tau_rows, 0, null, 0, top_p, null, min_p, null,
+                                       tokens, p, p, kept, kept_ld, ws, nbytes, null)
+
+    bad, unsupported = -1, -5
+    assert sample(N=0) == 0
+    assert sample(N=-1) == sample(V=0) == sample(ld=39) == sample(logits=null) == sample(u=null) == bad
+    assert sample(tokens=null) == sample(dtype=3) == sample(kept=p, kept_ld=1) == bad
+    assert sample(tau=-1.0) == sample(tau=math.nan) == sample(top_p=math.nan) == sample(min_p=-1.0) == bad
+    assert sample(ws=null) == sample(nbytes=100) == -3 and sample(ws=ctypes.c_void_p(4100)) == -2
+    assert sample(V=(1 << 22) + 1, ld=(1 << 22) + 1) == unsupported
+    assert lib.areal_sample_tokens_workspace_bytes(3, (1 << 22) + 1) == 0
+
+    def kept(dtype=1, ld=40, N=3, V=40, words=2, inv=1.0, k=p, lab=p):
+        a = lib.areal_kept_logprobs_entropy_fwd(p, dtype, ld, lab, k, words, N, V, inv, p, p, p, null)
+        b = lib.areal_kept_logprobs_entropy_bwd(p, dtype, ld, lab, k, words, N, V, inv, p, p, p, p, p, ld, null)
+        assert a == b
+        return a
+
+    assert kept(N=0) == 0
+    assert kept(ld=39) == kept(words=1) == kept(inv=0.0) == kept(inv=math.nan) == kept(k=null) == kept(lab=null) == bad
+    assert kept(dtype=3) == kept(N=-1) == kept(V=0) == bad and kept(V=(1 << 30) + 1, ld=1 << 31, words=1 << 26) == unsupported
+    assert lib.areal_kept_logprobs_entropy_bwd(p, 1, 40, p, p, 2, 3, 40, 1.0, p, null, p, p, p, 40, null) == bad
+
+    def fwd(w=p, wd=1, ldw=8, ids=p, T=4, H=8, V=6, od=1):
+        return lib.areal_embedding_fwd(w, wd, ldw, ids, T, H, V, 1.0, p, od, null)
+
+    assert fwd(T=0) == 0
+    assert fwd(w=null) == fwd(wd=3) == fwd(od=-1) == fwd(ldw=7) == fwd(ids=null) == fwd(H=0) == fwd(V=0) == fwd(T=-1) == bad
+    assert fwd(T=1 << 31) == fwd(V=1 << 31) == unsupported
+
+    def bwd(g=p, gd=1, T=4, H=8, V=6, dw=p, dd=1, add=0, ws=p, nbytes=None):
+        nbytes = lib.areal_embedding_bwd_workspace_bytes(T, H, V) if nbytes is None else nbytes
+        return lib.areal_embedding_bwd(g, gd, p, T, H, V, 1.0, -1, dw, dd, add, ws, nbytes, null)
+
+    assert bwd(T=0, dd=0, add=1) == 0
+    assert bwd(g=null) == bwd(gd=5) == bwd(dd=3) == bwd(dw=null) == bwd(H=0) == bwd(T=-1) == bad
+    assert bwd(add=1) == bwd(T=1 << 31) == unsupported
+    assert bwd(ws=null) == bwd(nbytes=10) == -3 and bwd(ws=ctypes.c_void_p(4100)) == -2
