@@ -9,6 +9,7 @@
 // (a value, and how many of its ties by index), found by radix selection over integer keys; masses in its histograms are
 // integers of 2^-s, whose sums do not depend on the order of the atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -17,21 +18,34 @@ namespace {
 constexpr int SEG = 1024;            // logits of one wave in the first pass
 constexpr int SEG_LANE = SEG / 64;   // per lane
 constexpr int SUBS = 16;             // maxima kept of a segment where top-k asks for them, one per four lanes
-constexpr int64_t MAX_SEGS = 4096;   // vocabularies up to 4 Mi
+constexpr int MAX_SEGS = 4096;       // vocabularies up to 4 Mi
+constexpr int FEW_SEGS = 512;        // up to 512 Ki
+constexpr unsigned MANY_SEGS = 16384;  // from here a wave takes four segments of the first pass
+constexpr int64_t FEW_ROWS = 256;
 constexpr int LIST = 4096;           // candidates held in LDS
 constexpr double LOG2E = 1.4426950408889634;
 
 // Logit types: VEC elements of 16 bytes, loaded from any element (unaligned access is enabled on gfx950).
 struct F32 {
   typedef float S;
+  typedef uint32_t B;
+  typedef f32x4 Reg;
   typedef f32x4 Vec __attribute__((aligned(4)));
+  static constexpr B NEG_INF = 0xff800000u;
+  static DEVI void put(f32x4& v, int j, B b) { v[j] = __builtin_bit_cast(float, b); }
   static constexpr int VEC = 4, LOW = 0;  // LOW: bits of an fp32 key that are the same for all values of the type
   static DEVI void widen(const f32x4& v, float* o) { o[0] = v[0]; o[1] = v[1]; o[2] = v[2]; o[3] = v[3]; }
   static DEVI float one(float v) { return v; }
 };
 struct BF16 {
   typedef u16 S;
+  typedef u16 B;
+  typedef u32x4 Reg;
   typedef u32x4 Vec __attribute__((aligned(2)));
+  static constexpr B NEG_INF = 0xff80;
+  static DEVI void put(u32x4& v, int j, B b) {
+    v[j / 2] = j & 1 ? (v[j / 2] & 0xffffu) | (uint32_t)b << 16 : (uint32_t)b;
+  }
   static constexpr int VEC = 8, LOW = 16;
   static DEVI void widen(const u32x4& v, float* o) {
 #pragma unroll
@@ -45,7 +59,11 @@ struct BF16 {
 struct FP16 {
   typedef _Float16 S;
   typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  typedef u16 B;
+  typedef f16x8 Reg;
   typedef f16x8 Vec __attribute__((aligned(2)));
+  static constexpr B NEG_INF = 0xfc00;
+  static DEVI void put(f16x8& v, int j, B b) { v[j] = __builtin_bit_cast(_Float16, b); }
   static constexpr int VEC = 8, LOW = 13;
   static DEVI void widen(const f16x8& v, float* o) {
 #pragma unroll
@@ -62,7 +80,7 @@ struct Call {
   const void* uniforms;
   const float *temperature_rows, *top_p_rows, *min_p_rows;
   const void* top_k_rows;
-  double temperature, top_p, min_p;
+  double temperature, rate, top_p, min_p;  // rate: log2(e) / temperature
   int64_t top_k;
   int wide_uniforms, wide_top_k, subs, fixed_bits;
   int64_t* tokens;
@@ -84,6 +102,9 @@ struct Settings {
   int64_t top_k;
   bool top1, greedy, bad;
 };
+__host__ DEVI double rate_of(double tau) {  // (finite: the largest logit has weight 1 at any temperature)
+  return tau <= 0. ? LOG2E : fmin(LOG2E / tau, 1e300);
+}
 DEVI Settings settings_of(const Call& a, int64_t row) {
   Settings s;
   const double tau = a.temperature_rows ? (double)a.temperature_rows[row] : a.temperature;
@@ -97,17 +118,15 @@ DEVI Settings settings_of(const Call& a, int64_t row) {
   s.greedy = tau <= 0.;
   s.top1 = s.greedy || s.top_k == 1 || s.top_p <= 0.;
   s.min_p = fmin(s.min_p, 1.);
-  s.c = s.greedy ? LOG2E : fmin(LOG2E / tau, 1e300);  // (finite: the largest logit has weight 1 at any temperature)
+  s.c = a.temperature_rows ? rate_of(tau) : a.rate;
   return s;
 }
 
-// 2^t for t <= 0. 2^f = 1 + f q(f) on [-1/2, 1/2], q interpolated at the Chebyshev nodes (relative error of 2^f 2.2e-12;
-// exactly 1 at 0): a token is drawn wrongly if its uniform number falls that close to a border, which at 150,000
-// tokens of equal weight happens to one row in 10^6. Results below 2^-1000 are taken as that.
-DEVI double exp2_low(double t) {
-  t = fmax(t, -1000.);
-  constexpr double MAGIC = 6755399441055744.;  // 1.5 * 2^52: the sum's low bits are the nearest integer
-  const double s = t + MAGIC, f = t - (s - MAGIC);
+// 2^f = 1 + f q(f) on [-1/2, 1/2], q interpolated at the Chebyshev nodes (relative error of 2^f 2.2e-12; exactly 1 at 0),
+// times 2^n, n the low 32 bits of `s`: a token is drawn wrongly if its uniform number falls that close to a border, which
+// at 150,000 tokens of equal weight happens to one row in 10^6.
+constexpr double ROUND = 6755399441055744.;  // 1.5 * 2^52: a sum with it has the nearest integer in its low bits
+DEVI double exp2_parts(double f, double s) {
   double q = 0x1.63b2d7960e61cp-20;
   q = fma(q, f, 0x1.00c0e4e159a42p-16);
   q = fma(q, f, 0x1.4308c7183e3d5p-13);
@@ -116,17 +135,22 @@ DEVI double exp2_low(double t) {
   q = fma(q, f, 0x1.c6b08da70cce4p-5);
   q = fma(q, f, 0x1.ebfbdff82a734p-3);
   q = fma(q, f, 0x1.62e42fef9cc69p-1);
-  const double r = fma(q, f, 1.);
-  int2 b = __builtin_bit_cast(int2, r);
-  b.y += __builtin_bit_cast(int2, s).x << 20;
+  int2 b = __builtin_bit_cast(int2, fma(q, f, 1.));
+  // (one instruction; written in C++ it becomes a 64-bit addition with its moves)
+  asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(b.y) : "v"(__builtin_bit_cast(int2, s).x));
   return __builtin_bit_cast(double, b);
 }
-// The same, and 0 from 2^-1000 down (also for a NaN, which -inf times a rate of 0 is).
+// 2^t for t <= 0; results below 2^-1000 are taken as that.
+DEVI double exp2_low(double t) {
+  t = fmax(t, -1000.);
+  const double s = t + ROUND;
+  return exp2_parts(t - (s - ROUND), s);
+}
+// exp((x - m) / temperature), and 0 from 2^-1000 down (also for a NaN, which -inf times a rate of 0 is).
 DEVI double weight_of(float x, double m, double c) {
   const double t = ((double)x - m) * c;
   return t > -1000. ? exp2_low(t) : 0.;
 }
-
 // Integers in the order of the floats; -0 and +0 are the same.
 DEVI uint32_t key_of(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
@@ -137,58 +161,102 @@ DEVI float value_of(uint32_t key) {
 }
 
 // Element g * VEC + j of a lane is logit base + (g * 64 + lane) * VEC + j; behind the row: -inf.
+template <class E>
+struct Raw {
+  typename E::Reg v[SEG_LANE / E::VEC];
+};
 template <class E, bool NT = false>
-DEVI void load_seg(const typename E::S* row, int base, int V, int lane, float (&x)[SEG_LANE]) {
+DEVI void load_raw(const typename E::S* row, int base, int V, int lane, Raw<E>& x) {
   constexpr int VEC = E::VEC, G = SEG_LANE / VEC;
   if (base + SEG <= V) {
-    typename E::Vec v[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const auto* const at = (const typename E::Vec*)(row + base + (g * 64 + lane) * VEC);
-      v[g] = NT ? __builtin_nontemporal_load(at) : *at;
+      x.v[g] = NT ? __builtin_nontemporal_load(at) : *at;
     }
-#pragma unroll
-    for (int g = 0; g < G; ++g) E::widen(v[g], x + g * VEC);
   } else {
 #pragma unroll
-    for (int i = 0; i < SEG_LANE; ++i) {
-      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
-      x[i] = at < V ? E::one(row[at]) : neg_inf();
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int at = base + (g * 64 + lane) * VEC + j;
+        E::put(x.v[g], j, at < V ? __builtin_bit_cast(typename E::B, row[at]) : E::NEG_INF);
+      }
     }
   }
 }
+template <class E>
+DEVI void widen_raw(const Raw<E>& r, float (&x)[SEG_LANE]) {
+#pragma unroll
+  for (int g = 0; g < SEG_LANE / E::VEC; ++g) E::widen(r.v[g], x + g * E::VEC);
+}
+template <class E, bool NT = false>
+DEVI void load_seg(const typename E::S* row, int base, int V, int lane, float (&x)[SEG_LANE]) {
+  Raw<E> r;
+  load_raw<E, NT>(row, base, V, lane, r);
+  widen_raw<E>(r, x);
+}
+// Index of element i (a constant) of the lane, from the segment's start.
+template <class E>
+DEVI int place_of(int i, int lane) { return ((i / E::VEC) * 64 + lane) * E::VEC + i % E::VEC; }
 
-// First pass, a wave per segment: its largest logit and the mass relative to that.
-template <class E, bool NT>
-__global__ __launch_bounds__(256) void sample_segments_kernel(Call a, unsigned units, int64_t row0) {
+// First pass, a wave per GROUP consecutive segments: the largest logit of each and the mass relative to that.
+template <class E, int GROUP>
+__global__ __launch_bounds__(256) void sample_segments_kernel(Call a, unsigned units, unsigned groups, int64_t row0) {
   const unsigned unit = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (unit >= units) return;
   const int lane = threadIdx.x & 63;
-  const unsigned r = unit / (unsigned)a.segs;
-  const int seg = (int)(unit - r * (unsigned)a.segs);
+  const unsigned r = unit / groups;
+  const int begin = (int)(unit - r * groups) * GROUP, end = min(begin + GROUP, a.segs);
   const int64_t row = row0 + r;
-  float x[SEG_LANE];
-  load_seg<E, NT>((const typename E::S*)a.logits + row * a.ld, seg * SEG, a.V, lane, x);
+  const auto* const x_row = (const typename E::S*)a.logits + row * a.ld;
+  Raw<E> now, next;
+  load_raw<E>(x_row, begin * SEG, a.V, lane, now);
   const Settings s = settings_of(a, row);
-  float mx = x[0];
+  const double below = 1000. / s.c;
+#pragma unroll 1
+  for (int seg = begin; seg < end; ++seg) {
+    if (GROUP > 1 && seg + 1 < end) load_raw<E>(x_row, (seg + 1) * SEG, a.V, lane, next);
+    float x[SEG_LANE];
+    widen_raw<E>(now, x);
+    float mx = x[0];
 #pragma unroll
-  for (int i = 1; i < SEG_LANE; ++i) mx = stat_max(mx, x[i]);  // a NaN stays
-  if (a.subs) {
-    float q = stat_max(mx, dpp_move<0xb1>(mx, mx));  // quad_perm [1,0,3,2]
-    q = stat_max(q, dpp_move<0x4e>(q, q));           // quad_perm [2,3,0,1]
-    if ((lane & 3) == 0) a.sub_max[(int64_t)unit * SUBS + (lane >> 2)] = q;
-  }
-  mx = wave_stat_max(mx);
-  double sum = 0.;
-  if (mx > neg_inf()) {  // (rows with a NaN or +inf come out bad whatever their sums are)
-    const double m = mx;
+    for (int i = 1; i < SEG_LANE; ++i) mx = stat_max(mx, x[i]);  // a NaN stays
+    const int64_t at = (int64_t)r * a.segs + seg;
+    if (a.subs) {
+      float q = stat_max(mx, dpp_move<0xb1>(mx, mx));  // quad_perm [1,0,3,2]
+      q = stat_max(q, dpp_move<0x4e>(q, q));           // quad_perm [2,3,0,1]
+      if ((lane & 3) == 0) a.sub_max[at * SUBS + (lane >> 2)] = q;
+    }
+    mx = wave_stat_max(mx);
+    double sum = 0.;
+    if (mx > neg_inf()) {  // (rows with a NaN or +inf come out bad whatever their sums are)
+      const double m = mx;
+      if (s.c > 1e-20 && fabs(m * s.c) < 1e9) {
+        // The exponent z * c as its nearest integer and the rest, one fma each. Logits 1000 binades and more below the
+        // maximum are taken as that (at such m * c steps of fp32 near the maximum are up to 120 binades, so no nearer ones).
+        const float lowest = (float)(m - below);
 #pragma unroll
-    for (int i = 0; i < SEG_LANE; ++i) sum += exp2_low(((double)x[i] - m) * s.c);
-    sum = wave_sum(sum);
-  }
-  if (lane == 0) {
-    a.seg_max[unit] = mx;
-    a.seg_sum[unit] = sum;
+        for (int i = 0; i < SEG_LANE; ++i) {
+          const double z = (double)stat_max(x[i], lowest) - m, n = fma(z, s.c, ROUND);
+          sum += exp2_parts(fma(z, s.c, ROUND - n), n);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < SEG_LANE; ++i) {
+          float v = x[0];
+#pragma unroll
+          for (int j = 1; j < SEG_LANE; ++j) v = i == j ? x[j] : v;
+          sum += exp2_low(((double)v - m) * s.c);
+        }
+      }
+      sum = wave_sum(sum);
+    }
+    if (lane == 0) {
+      a.seg_max[at] = mx;
+      a.seg_sum[at] = sum;
+    }
+    now = next;
   }
 }
 
@@ -213,13 +281,10 @@ struct BlockScan {
   }
 };
 
-struct Picked {
-  int index;    // -1: no element with a weight
-  bool inside;  // the target lies in it (else: the last with a weight)
-};
-// The first element in index order whose running sum (from `base`) passes `target`, by one wave.
+// The first element in index order whose running sum (from `base`) passes `target`, else the last with a weight; by one
+// wave.
 template <class E>
-DEVI Picked wave_pick(const double (&w)[SEG_LANE], int seg_base, double base, double target, int lane) {
+DEVI int wave_pick(const double (&w)[SEG_LANE], int seg_base, double base, double target, int lane) {
   constexpr int VEC = E::VEC, G = SEG_LANE / VEC;
   int last = -1;
 #pragma unroll
@@ -229,12 +294,11 @@ DEVI Picked wave_pick(const double (&w)[SEG_LANE], int seg_base, double base, do
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       s += w[g * VEC + j];
-      if (w[g * VEC + j] > 0.) mine = seg_base + (g * 64 + lane) * VEC + j;
+      if (w[g * VEC + j] > 0.) mine = seg_base + place_of<E>(g * VEC + j, lane);
     }
     const double incl = wave_inclusive_scan(s, 0., [](double x, double y) { return x + y; });
     const unsigned long long cross = __builtin_amdgcn_ballot_w64(s > 0. && base + incl > target);
     if (cross != 0) {
-      const int at = __builtin_ctzll(cross);
       double cum = base + wave_shift_up(incl, 0.);
       int found = mine;  // rounding may leave it to the lane's last
       bool open = true;
@@ -242,25 +306,25 @@ DEVI Picked wave_pick(const double (&w)[SEG_LANE], int seg_base, double base, do
       for (int j = 0; j < VEC; ++j) {
         cum += w[g * VEC + j];
         if (open && w[g * VEC + j] > 0. && cum > target) {
-          found = seg_base + (g * 64 + lane) * VEC + j;
+          found = seg_base + place_of<E>(g * VEC + j, lane);
           open = false;
         }
       }
-      return {__builtin_amdgcn_readlane(found, at), true};
+      return __builtin_amdgcn_readlane(found, __builtin_ctzll(cross));
     }
     const unsigned long long any = __builtin_amdgcn_ballot_w64(mine >= 0);
     if (any != 0) last = __builtin_amdgcn_readlane(mine, 63 - __builtin_clzll(any));
     base += lane_value(incl, 63);
   }
-  return {last, false};
+  return last;
 }
 
-// Positions of flagged elements (bit g * VEC + j of `flags`) in index order: starts[g] of a lane's first in group g,
-// counted from `base`. Returns the wave's number of them.
+// Positions of flagged elements (bit i of `flags`: element i of the lane) in index order: starts[g] of a lane's first in
+// group g. Returns the wave's number of them.
 template <class E>
-DEVI int order_in_wave(unsigned flags, int base, int (&starts)[SEG_LANE / E::VEC]) {
+DEVI int order_in_wave(unsigned flags, int (&starts)[SEG_LANE / E::VEC]) {
   constexpr int VEC = E::VEC, G = SEG_LANE / VEC;
-  int at = base;
+  int at = 0;
 #pragma unroll
   for (int g = 0; g < G; ++g) {
     const int n = __popc((flags >> (g * VEC)) & ((1u << VEC) - 1));
@@ -268,119 +332,105 @@ DEVI int order_in_wave(unsigned flags, int base, int (&starts)[SEG_LANE / E::VEC
     starts[g] = at + incl - n;
     at += lane_value(incl, 63);
   }
-  return at - base;
+  return at;
+}
+template <class E>
+DEVI int order_of(unsigned flags, const int (&starts)[SEG_LANE / E::VEC], int i) {
+  constexpr int VEC = E::VEC;
+  return starts[i / VEC] + __popc((flags >> (i / VEC * VEC)) & ((1u << (i % VEC)) - 1));
 }
 
-// A row's cut and its token, one workgroup a row.
+// ---- second pass, a workgroup per row ----
 template <int THREADS>
 struct RowShared {
-  static constexpr int WAVES = THREADS / 64;
-  BlockScan<WAVES, double> scan_f64;
-  BlockScan<WAVES, int> scan_int;
-  unsigned long long mass[256];
-  uint32_t count[256];
-  union {
-    struct {
-      uint32_t key[LIST];
-      int index[LIST];
-    } list;
-    struct {
-      double mass[MAX_SEGS];
-      int ties[MAX_SEGS];
-    } seg;
-  };
-  unsigned short active[MAX_SEGS];
-  unsigned long long above;
-  int bin, ties, first, last, wave_count[WAVES];
-  uint32_t low_key;
-  int cut_index;
-  float xmax[WAVES];
+  BlockScan<THREADS / 64, double> scan;
+  float xmax[THREADS / 64];
+  int first, last;
   double target;
 };
+constexpr int NO_INDEX = 0x7fffffff;
 
+// A row's segments in the hands of THREADS threads, `per` consecutive ones each.
 template <class E, int THREADS>
-__global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t row0) {
-  constexpr int VEC = E::VEC, G = SEG_LANE / VEC, WAVES = THREADS / 64, LOW = E::LOW;
-  __shared__ RowShared<THREADS> sh;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const unsigned r = blockIdx.x;
-  const int64_t row = row0 + r;
-  const typename E::S* x_row = (const typename E::S*)a.logits + row * a.ld;
-  const float* seg_max = a.seg_max + (int64_t)r * a.segs;
-  const double* seg_sum = a.seg_sum + (int64_t)r * a.segs;
-  const Settings s = settings_of(a, row);
-  double u = a.wide_uniforms ? ((const double*)a.uniforms)[row] : (double)((const float*)a.uniforms)[row];
-  u = fmin(fmax(u, 0.), 1.);
+struct Row {
+  static constexpr int WAVES = THREADS / 64;
+  const Call& a;
+  RowShared<THREADS>& sh;
+  const int tid, lane, wave;
+  const unsigned r;
+  const int64_t row;
+  const typename E::S* const x_row;
+  const float* const seg_max;
+  const double* const seg_sum;
+  const Settings s;
+  int begin, end;
+  float top;
+  double m, u, all_mass, before;
 
-  const int per = (a.segs + THREADS - 1) / THREADS;  // segments of a thread, in order
-  const int seg_begin = min(tid * per, a.segs), seg_end = min(seg_begin + per, a.segs);
-  float mx = neg_inf();
-  for (int i = seg_begin; i < seg_end; ++i) mx = stat_max(mx, seg_max[i]);
-  mx = wave_stat_max(mx);
-  if (lane == 0) sh.xmax[wave] = mx;
-  if (tid == 0) {
-    sh.first = 0x7fffffff;
-    sh.last = -1;
-    sh.low_key = 0xffffffffu;
-    sh.cut_index = -1;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) mx = stat_max(mx, sh.xmax[i]);
-  if (s.bad || !(mx < pos_inf()) || !(mx > neg_inf())) {  // NaN, +inf, or nothing but -inf
+  DEVI Row(const Call& call, RowShared<THREADS>& shared, int64_t row0)
+      : a(call), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), r(blockIdx.x),
+        row(row0 + blockIdx.x), x_row((const typename E::S*)a.logits + row * a.ld),
+        seg_max(a.seg_max + (int64_t)r * a.segs), seg_sum(a.seg_sum + (int64_t)r * a.segs), s(settings_of(a, row)) {}
+
+  DEVI double seg_mass(int i) const { return seg_sum[i] * weight_of(seg_max[i], m, s.c); }
+
+  // Largest logit and mass of the row. False: there is no distribution (and the outputs say so).
+  DEVI bool combine() {
+    u = a.wide_uniforms ? ((const double*)a.uniforms)[row] : (double)((const float*)a.uniforms)[row];
+    u = fmin(fmax(u, 0.), 1.);
+    const int per = (a.segs + THREADS - 1) / THREADS;
+    begin = min(tid * per, a.segs);
+    end = min(begin + per, a.segs);
+    top = neg_inf();
+    for (int i = begin; i < end; ++i) top = stat_max(top, seg_max[i]);
+    top = wave_stat_max(top);
     if (tid == 0) {
-      a.tokens[row] = -1;
-      a.logprobs[row] = a.full_logprobs[row] = __builtin_nanf("");
-      a.cut[r] = pos_inf();
-      a.cut_index[r] = -1;
+      sh.first = NO_INDEX;
+      sh.last = -1;
     }
-    return;
+    if (WAVES > 1) {
+      if (lane == 0) sh.xmax[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) top = stat_max(top, sh.xmax[i]);
+    } else {
+      __syncthreads();
+    }
+    if (s.bad || !(top < pos_inf()) || !(top > neg_inf())) {  // NaN, +inf, or nothing but -inf
+      if (tid == 0) {
+        a.tokens[row] = -1;
+        a.logprobs[row] = a.full_logprobs[row] = __builtin_nanf("");
+        a.cut[r] = pos_inf();
+        a.cut_index[r] = -1;
+      }
+      return false;
+    }
+    m = top;
+    double own = 0.;
+    for (int i = begin; i < end; ++i) own += seg_mass(i);
+    before = sh.scan.exclusive(own, all_mass);
+    return true;
   }
-  const double m = mx;
-  double own = 0.;
-  for (int i = seg_begin; i < seg_end; ++i) own += seg_sum[i] * weight_of(seg_max[i], m, s.c);
-  double all_mass;
-  const double before = sh.scan_f64.exclusive(own, all_mass);
 
-  // Results, by thread 0. z: the mass of the kept set.
-  auto finish = [&](int token, double z, float cut, int cut_index) {
-    const double d = ((double)E::one(x_row[token]) - m) * s.c;
+  // Results, by one thread. z: the mass of the kept set.
+  DEVI void finish(int token, double z, float cut, int cut_index) const {
     constexpr double LN2 = 0.6931471805599453;
+    const double d = ((double)E::one(x_row[token]) - m) * s.c;
     a.tokens[row] = token;
     a.logprobs[row] = (float)(s.top1 ? 0. : fma(d, LN2, -log(z)));
     a.full_logprobs[row] = (float)(s.greedy ? 0. : fma(d, LN2, -log(all_mass)));
     a.cut[r] = cut;
     a.cut_index[r] = cut_index;
-  };
-
-  if (s.top1) {  // the lowest index of the largest logit
-    for (int i = seg_begin; i < seg_end; ++i)
-      if (seg_max[i] == mx) {
-        atomicMin(&sh.first, i);
-        break;
-      }
-    __syncthreads();
-    if (wave == 0) {
-      const int seg = sh.first;
-      float x[SEG_LANE];
-      load_seg<E>(x_row, seg * SEG, a.V, lane, x);
-      int at = 0x7fffffff;
-#pragma unroll
-      for (int i = SEG_LANE - 1; i >= 0; --i)
-        if (x[i] == mx) at = seg * SEG + ((i / VEC) * 64 + lane) * VEC + i % VEC;
-      at = wave_reduce(at, [](int p, int q) { return p < q ? p : q; });
-      if (lane == 0) finish(at, 1., mx, at);
-    }
-    return;
   }
 
-  const bool use_k = s.top_k < a.V, use_p = s.top_p < 1., use_min = s.min_p > 0.;
-  if (!use_k && !use_p && !use_min) {  // the whole distribution: only the segment with the target is read again
-    const double target = u * all_mass;
-    double cum = before;
-    for (int i = seg_begin; i < seg_end; ++i) {
-      const double w = seg_sum[i] * weight_of(seg_max[i], m, s.c);
-      if (w > 0.) {
+  // Which of n consecutive masses the target lies in, a run [i0, i1) of them with a thread; sh.target = their sum in front
+  // of it. All threads get it.
+  template <class F>
+  DEVI int choose(int i0, int i1, double front, double target, F mass) {
+    double cum = front;
+    for (int i = i0; i < i1; ++i) {
+      const double w = mass(i);
+      if (w > 1e-200) {  // (a segment without a kept logit may have a mass of 1024 times 2^-1000)
         if (cum + w > target) {
           atomicMin(&sh.first, i);
           break;
@@ -390,71 +440,175 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       cum += w;
     }
     __syncthreads();
-    const int seg = sh.first != 0x7fffffff ? sh.first : sh.last;
-    if (seg >= seg_begin && seg < seg_end) {
-      double c2 = before;
-      for (int i = seg_begin; i < seg; ++i) c2 += seg_sum[i] * weight_of(seg_max[i], m, s.c);
-      sh.target = c2;
+    const int at = sh.first != NO_INDEX ? sh.first : sh.last;
+    if (at >= i0 && at < i1) {
+      cum = front;
+      for (int i = i0; i < at; ++i) cum += mass(i);
+      sh.target = cum;
     }
     __syncthreads();
+    return at;
+  }
+
+  // The settings that need no selection. False: others.
+  DEVI bool simple() {
+    if (s.top1) {  // the lowest index of the largest logit
+      for (int i = begin; i < end; ++i)
+        if (seg_max[i] == top) {
+          atomicMin(&sh.first, i);
+          break;
+        }
+      __syncthreads();
+      if (wave == 0) {
+        const int seg = sh.first;
+        float x[SEG_LANE];
+        load_seg<E>(x_row, seg * SEG, a.V, lane, x);
+        int at = NO_INDEX;
+#pragma unroll
+        for (int i = SEG_LANE - 1; i >= 0; --i)
+          if (x[i] == top) at = seg * SEG + place_of<E>(i, lane);
+        at = wave_reduce(at, [](int p, int q) { return p < q ? p : q; });
+        if (lane == 0) finish(at, 1., top, at);
+      }
+      return true;
+    }
+    if (s.top_k < a.V || s.top_p < 1. || s.min_p > 0.) return false;
+    // the whole distribution: only the segment with the target is read again
+    const double target = u * all_mass;
+    const int seg = choose(begin, end, before, target, [&](int i) { return seg_mass(i); });
     if (wave == 0) {
       float x[SEG_LANE];
       double w[SEG_LANE];
       load_seg<E>(x_row, seg * SEG, a.V, lane, x);
 #pragma unroll
       for (int i = 0; i < SEG_LANE; ++i) w[i] = weight_of(x[i], m, s.c);
-      const Picked p = wave_pick<E>(w, seg * SEG, sh.target, target, lane);
-      if (lane == 0) finish(p.index, all_mass, neg_inf(), -1);
+      const int token = wave_pick<E>(w, seg * SEG, sh.target, target, lane);
+      if (lane == 0) finish(token, all_mass, neg_inf(), -1);
     }
-    return;
+    return true;
   }
+};
 
-  // ---- a lower bound on the kept logits, so that few candidates are looked at ----
-  // clears the counts, then `add` fills them; the descending bin in which the running count reaches `want`
-  auto select_bin = [&](int64_t want) {
+// Calls without a limit in any row.
+template <class E>
+__global__ __launch_bounds__(256) void sample_whole_kernel(Call a, int64_t row0) {
+  __shared__ RowShared<256> sh;
+  Row<E, 256> row(a, sh, row0);
+  if (row.combine()) row.simple();
+}
+
+constexpr int BINS = 2048;
+template <int THREADS, int SEGS>
+struct CutShared {
+  static constexpr int WAVES = THREADS / 64;
+  RowShared<THREADS> row;
+  BlockScan<WAVES, int> ints;
+  BlockScan<WAVES, unsigned long long> wide;
+  union {
+    unsigned long long mass[256];
+    uint32_t count[256];
+  };
+  unsigned long long above;
+  int bin, ties, bin_low, bin_high, cut_index;
+  int wave_count[2][WAVES];
+  unsigned short active[SEGS];
+  int seg_first[SEGS];  // of an active segment: entries of the list before its own, or ties
+  uint32_t key[LIST];   // the list, in index order
+  int index[LIST];
+  union {
+    unsigned long long bins[BINS];
+    double seg_mass[SEGS];
+  };
+};
+
+// The others. The kept set is a prefix of the order: it ends at a key (`cut_key`) and at an index among that key's ties.
+template <class E, int THREADS, int SEGS>
+__global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t row0) {
+  constexpr int VEC = E::VEC, G = SEG_LANE / VEC, WAVES = THREADS / 64, LOW = E::LOW;
+  __shared__ CutShared<THREADS, SEGS> sh;
+  Row<E, THREADS> row(a, sh.row, row0);
+  if (!row.combine() || row.simple()) return;
+  const Settings& s = row.s;
+  const int tid = row.tid, lane = row.lane, wave = row.wave;
+  const double m = row.m, c = s.c;
+  const float top = row.top;
+  const bool use_k = s.top_k < a.V, use_p = s.top_p < 1., use_min = s.min_p > 0.;
+  const uint32_t top_key = key_of(top);
+  if (tid == 0) sh.cut_index = NO_INDEX;
+  // The first key from 0 to top_key for which `reached` holds, which it does from some key on (and at top_key): 64 probes
+  // a round, by every wave for itself.
+  auto first_key = [&](auto reached) {
+    uint32_t from = 0, to = top_key;  // the answer lies in [from, to]
+    while (from < to) {
+      const uint32_t step = (to - from) / 64 + 1;
+      const uint64_t probe64 = (uint64_t)from + (uint64_t)step * lane;
+      const uint32_t probe = probe64 < to ? (uint32_t)probe64 : to;
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(reached(probe));
+      const int at = __builtin_ctzll(hit | 1ull << 63);  // (the last probe is reached or below the answer by a step at most)
+      const bool any = hit != 0;
+      const uint32_t found = __builtin_amdgcn_readlane(probe, at);
+      if (!any) {
+        from = found + 1;
+      } else {
+        const uint32_t before = at == 0 ? from : __builtin_amdgcn_readlane(probe, at - 1) + 1;
+        from = before;
+        to = found;
+      }
+    }
+    return to;
+  };
+
+  auto clear_bins = [&] {  // 256 of them
+    __syncthreads();
+    for (int i = tid; i < 256; i += THREADS) sh.mass[i] = 0;
+    __syncthreads();
+  };
+  // the bin, from the 256th downwards, in which the running count reaches `want`: sh.bin, the count in front and its own
+  auto find_count = [&](int64_t want) {
     __syncthreads();
     if (wave == 0) {
-      uint32_t c[4];
+      uint32_t n4[4];
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) n += (int)(c[i] = sh.count[255 - 4 * lane - i]);
+      for (int i = 0; i < 4; ++i) n += (int)(n4[i] = sh.count[255 - 4 * lane - i]);
       const int incl = wave_inclusive_scan(n, 0, [](int x, int y) { return x + y; });
       if (incl - n < want && incl >= want) {
         int cum = incl - n;
         bool open = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (open && cum + (int)c[i] >= want) {
+          if (open && cum + (int)n4[i] >= want) {
             sh.bin = 255 - 4 * lane - i;
             sh.above = (unsigned long long)cum;
-            sh.ties = (int)c[i];
+            sh.ties = (int)n4[i];
             open = false;
           }
-          cum += (int)c[i];
+          cum += (int)n4[i];
         }
       }
     }
     __syncthreads();
   };
-  auto clear_bins = [&] {
-    __syncthreads();
-    for (int i = tid; i < 256; i += THREADS) {
-      sh.count[i] = 0;
-      sh.mass[i] = 0;
-    }
-    __syncthreads();
-  };
-  const uint32_t top_key = key_of(mx);
+
+  // ---- a lower bound on the kept logits, so that few are looked at ----
   double bound = -1.7e308;
   // No token lighter than this is in S2: all those together weigh less than (1 - top_p) of the mass.
-  if (use_p && !use_k) bound = fmax(bound, m + log2((1. - s.top_p) * all_mass / a.V) / s.c);
-  if (use_min && !(use_k && use_p)) bound = fmax(bound, m + log2(s.min_p) / s.c);  // (else S1's whole mass is needed)
-  bound -= 1e-6 * fabs(bound) + 1e-6 / s.c;
+  if (use_p && !use_k) bound = fmax(bound, m + log2((1. - s.top_p) * row.all_mass / a.V) / c);
+  bound -= 1e-6 * fabs(bound) + 1e-6 / c;
   float low = bound > -3.4e38 ? (float)bound : -3.402823466e38f;
-  if (use_k && a.subs && s.top_k <= (int64_t)a.segs * SUBS) {
+  // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
+  const uint32_t min_key =
+      use_min ? first_key([&](uint32_t key) {
+        const float x = value_of(key);
+        return x == x && weight_of(x, m, c) >= s.min_p;  // (the lowest keys are NaN's, and -inf's)
+      })
+              : 0;
+  const bool min_last = use_k && use_p;
+  if (use_min && !min_last) low = fmaxf(low, value_of(min_key));
+  if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
     // top_k maxima of disjoint parts of the row are that many logits: the top_k-th largest of the row is no lower than
     // theirs. Its upper 16 bits are enough.
-    const float* subs = a.sub_max + (int64_t)r * a.segs * SUBS;
+    const float* subs = a.sub_max + (int64_t)row.r * a.segs * SUBS;
     const int n = a.segs * SUBS;
     uint32_t prefix = 0;
     int64_t want = s.top_k;
@@ -465,7 +619,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
         const uint32_t key = key_of(subs[i]);
         if (shift == 24 || (key >> 24) == (prefix >> 24)) atomicAdd(&sh.count[(key >> shift) & 255], 1u);
       }
-      select_bin(want);
+      find_count(want);
       prefix |= (uint32_t)sh.bin << shift;
       want -= (int64_t)sh.above;
     }
@@ -473,93 +627,110 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
     if (lowest > low) low = lowest;  // (not where it is a NaN's pattern, below that of -inf)
   }
 
-  // ---- the segments and the logits that reach it, in index order ----
-  int mine = 0;
-  for (int i = seg_begin; i < seg_end; ++i) mine += seg_max[i] >= low;
+  // ---- the segments that reach it, in index order ----
   int n_active;
-  int at = sh.scan_int.exclusive(mine, n_active);
-  for (int i = seg_begin; i < seg_end; ++i)
-    if (seg_max[i] >= low) sh.active[at++] = (unsigned short)i;
-  __syncthreads();
-  int n_cand = 0;
-  for (int i0 = 0; i0 < n_active; i0 += WAVES) {
-    float x[SEG_LANE];
-    unsigned flags = 0;
-    int base = 0;
-    if (i0 + wave < n_active) {
-      base = (int)sh.active[i0 + wave] * SEG;
-      load_seg<E>(x_row, base, a.V, lane, x);
-#pragma unroll
-      for (int i = 0; i < SEG_LANE; ++i) flags |= (x[i] >= low ? 1u : 0u) << i;
-    }
-    int starts[G];
-    const int n = order_in_wave<E>(flags, 0, starts);
-    if (lane == 0) sh.wave_count[wave] = n;
+  {
+    int mine = 0;
+    for (int i = row.begin; i < row.end; ++i) mine += row.seg_max[i] >= low;
+    int at = sh.ints.exclusive(mine, n_active);
+    for (int i = row.begin; i < row.end; ++i)
+      if (row.seg_max[i] >= low) sh.active[at++] = (unsigned short)i;
     __syncthreads();
-    int to = n_cand;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w == wave) to = n_cand;
-      n_cand += sh.wave_count[w];
+  }
+  auto load_active = [&](int i, Raw<E>& x) { load_raw<E>(row.x_row, (int)sh.active[i] * SEG, a.V, lane, x); };
+  // f(logits, i) of active segment i, a wave each; the next one's loads are under way meanwhile
+  auto sweep = [&](auto f) {
+    Raw<E> now, next;
+    if (wave < n_active) load_active(wave, now);
+    for (int i = wave; i < n_active; i += WAVES) {
+      if (i + WAVES < n_active) load_active(i + WAVES, next);
+      float x[SEG_LANE];
+      widen_raw<E>(now, x);
+      f(x, i);
+      now = next;
     }
-    if (flags != 0) {
+  };
+  // Puts the logits that flags_of(logits, i) marks into the list, in index order, and the number of them in front of each
+  // active segment into seg_first. Returns their number; one of more than LIST as soon as it is.
+  auto collect = [&](auto flags_of) {
+    int n = 0;
+    Raw<E> now, next;
+    if (wave < n_active) load_active(wave, now);
+    for (int i0 = 0, half = 0; i0 < n_active; i0 += WAVES, half ^= 1) {
+      const int i = i0 + wave;
+      float x[SEG_LANE];
+      unsigned flags = 0;
+      if (i + WAVES < n_active) load_active(i + WAVES, next);
+      widen_raw<E>(now, x);
+      if (i < n_active) flags = flags_of(x, i);
+      int starts[G];
+      const int own = order_in_wave<E>(flags, starts);
+      if (lane == 0) sh.wave_count[half][wave] = own;
+      __syncthreads();  // (the other half's readers are behind the next one)
+      int to = n;
 #pragma unroll
-      for (int i = 0; i < SEG_LANE; ++i) {
-        if (flags >> i & 1) {
-          const int p = to + starts[i / VEC] + __popc((flags >> (i / VEC * VEC)) & ((1u << (i % VEC)) - 1));
-          if (p < LIST) {
-            sh.list.key[p] = key_of(x[i]);
-            sh.list.index[p] = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) to += sh.wave_count[half][w];
+        n += sh.wave_count[half][w];
+      }
+      if (lane == 0 && i < n_active) sh.seg_first[i] = to;
+      if (flags != 0) {
+        const int base = (int)sh.active[i] * SEG;
+#pragma unroll
+        for (int j = 0; j < SEG_LANE; ++j) {
+          const int p = to + order_of<E>(flags, starts, j);
+          if ((flags >> j & 1) && p < LIST) {
+            sh.key[p] = key_of(x[j]);
+            sh.index[p] = base + place_of<E>(j, lane);
           }
         }
       }
+      if (n > LIST) break;
+      now = next;
     }
     __syncthreads();
-  }
-  const bool listed = n_cand <= LIST;
+    return n;
+  };
 
-  // f(key) of every candidate, in any order
-  auto each = [&](auto f) {
+  // ---- selection among candidates: the list, or the active segments' logits from `low` on ----
+  bool listed = true;
+  int n_list = 0;
+  auto each = [&](auto f) {  // f(key), in any order
     if (listed) {
-      for (int i = tid; i < n_cand; i += THREADS) f(sh.list.key[i]);
+      for (int i = tid; i < n_list; i += THREADS) f(sh.key[i]);
     } else {
-      for (int i = wave; i < n_active; i += WAVES) {
-        float x[SEG_LANE];
-        load_seg<E>(x_row, (int)sh.active[i] * SEG, a.V, lane, x);
+      sweep([&](const float (&x)[SEG_LANE], int) {
 #pragma unroll
         for (int j = 0; j < SEG_LANE; ++j)
           if (x[j] >= low) f(key_of(x[j]));
-      }
+      });
     }
   };
-  // Bits in which the candidates' keys can differ, downwards from `top_bits`.
+  // Bits in which candidates' keys can differ: those below `top_bits`, and not the type's own lowest.
   const uint32_t low_key = key_of(low);
   const int top_bits = low_key == top_key ? 0 : 32 - __builtin_clz(low_key ^ top_key);
-  auto whole_key = [&](uint32_t prefix) {  // the type's own lowest bits: 0, or of negative values 1
-    return prefix | ((prefix >> 31) ? 0u : (1u << LOW) - 1);
-  };
+  const uint32_t common = top_bits == 32 ? 0 : ~0u << top_bits;
+  auto whole_key = [&](uint32_t prefix) { return prefix | ((prefix >> 31) ? 0u : (1u << LOW) - 1); };
 
-  // ---- top-k: the key of the last logit of S1 and how many of its ties are in ----
-  uint32_t cut_key = 0;
-  int take = 0x7fffffff;
-  unsigned long long tied_out = 0;  // mass of the ties of cut_key that are not in S1
-  const bool cut_k = use_k && n_cand > s.top_k;
+  uint32_t cut_key = 0;  // kept: keys above it, and of its ties the first `take`
+  int take = NO_INDEX;
+  unsigned long long tied_out = 0;  // mass of the ties of cut_key that top-k leaves out
   const double unit = (double)(1ull << a.fixed_bits);
   auto fixed_mass = [&](uint32_t key) {  // 2^52 plus it has it in the low bits, rounded
-    const double w = fma(weight_of(value_of(key), m, s.c), unit, 4503599627370496.);
+    const double w = fma(weight_of(value_of(key), m, c), unit, 4503599627370496.);
     return __builtin_bit_cast(unsigned long long, w) & 0xfffffffffffffull;
   };
-  if (cut_k) {
-    uint32_t mask = top_bits == 32 ? 0 : ~0u << top_bits, prefix = top_key & mask;
-    int64_t want = s.top_k;
-    int ties = n_cand;
+  // The key of the want-th largest candidate.
+  auto select_count = [&](int64_t want, int n) {
+    uint32_t mask = common, prefix = top_key & common;
+    int ties = n;
     for (int bits = top_bits; bits > LOW;) {
       const int shift = max(bits - 8, LOW);
       clear_bins();
       each([&](uint32_t key) {
         if ((key & mask) == prefix) atomicAdd(&sh.count[(key >> shift) & ((1u << (bits - shift)) - 1)], 1u);
       });
-      select_bin(want);
+      find_count(want);
       prefix |= (uint32_t)sh.bin << shift;
       mask = ~0u << shift;
       want -= (int64_t)sh.above;
@@ -569,13 +740,11 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
     cut_key = whole_key(prefix);
     take = (int)want;
     tied_out = (unsigned long long)(ties - take) * fixed_mass(cut_key);
-  }
-
-  // ---- top-p inside S1 ----
-  if (use_p) {
-    uint32_t mask = top_bits == 32 ? 0 : ~0u << top_bits, prefix = top_key & mask;
+  };
+  // The key at which the candidates' mass reaches `least` (0: top_p of S1's), within S1.
+  auto select_mass = [&](double least) {
+    uint32_t mask = common, prefix = top_key & common;
     unsigned long long want = 0;
-    bool found = true;
     int bits = top_bits;
     bool first = true;
     do {
@@ -587,15 +756,15 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       });
       __syncthreads();
       if (wave == 0) {
-        unsigned long long c[4], n = 0;
+        unsigned long long n4[4], n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += c[i] = sh.mass[255 - 4 * lane - i];
+        for (int i = 0; i < 4; ++i) n += n4[i] = sh.mass[255 - 4 * lane - i];
         const unsigned long long incl =
             wave_inclusive_scan(n, 0ull, [](unsigned long long x, unsigned long long y) { return x + y; });
-        if (first) {  // in S2: what has less than top_p of S1's mass in front of it
-          const double z1 = use_k ? (double)(lane_value(incl, 63) - tied_out) : all_mass * unit;
-          want = (unsigned long long)ceil(s.top_p * z1);
-          if (want == 0) want = 1;
+        if (first) {  // in S2: what has less than this in front of it
+          const double least_fixed =
+              use_k ? s.top_p * (double)(lane_value(incl, 63) - tied_out) : least * unit;
+          want = least_fixed > 1. ? (unsigned long long)ceil(least_fixed) : 1;
         }
         if (lane == 0) sh.bin = -1;
         if (incl - n < want && incl >= want) {
@@ -603,194 +772,274 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
           bool open = true;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (open && cum + c[i] >= want) {
+            if (open && cum + n4[i] >= want) {
               sh.bin = 255 - 4 * lane - i;
               sh.above = want - cum;
               open = false;
             }
-            cum += c[i];
+            cum += n4[i];
           }
         }
       }
       __syncthreads();
       first = false;
-      if (sh.bin < 0) {  // less mass than that among the candidates: all of them stay
-        found = false;
-        break;
-      }
+      if (sh.bin < 0) return;  // less mass than that among the candidates: all of them stay
       prefix |= (uint32_t)sh.bin << shift;
       mask = ~0u << shift;
       want = sh.above;
       bits = shift;
     } while (bits > LOW);
-    if (found) {
-      const uint32_t key = whole_key(prefix);
-      const unsigned long long w = fixed_mass(key);
-      const int ties = w == 0 ? 0x7fffffff : (int)min((want + w - 1) / w, 0x7fffffffull);
-      take = key == cut_key ? min(take, ties) : ties;
-      cut_key = key;
+    const uint32_t key = whole_key(prefix);
+    const unsigned long long w = fixed_mass(key);
+    const int ties = w == 0 ? NO_INDEX : (int)min((want + w - 1) / w, (unsigned long long)NO_INDEX);
+    take = key == cut_key ? min(take, ties) : ties;
+    cut_key = key;
+  };
+  auto apply_min_p = [&] {
+    if (min_last && min_key > cut_key) {
+      cut_key = min_key;
+      take = NO_INDEX;
     }
-  }
-
-  // ---- the token, in index order; and the cut of the kept set ----
-  // kept: key > cut_key, or among the first `take` of its ties; and heavy enough
-  if (listed) {
-    constexpr int PER = LIST / THREADS;
-    const int i0 = tid * PER;
-    double w[PER];
-    int tied = 0;
+  };
+  constexpr int PER = LIST / THREADS;  // list entries of a thread, in order
+  // sh.cut_index: where the first `take` ties of cut_key in the list end
+  auto end_of_ties = [&] {
+    int tied = 0, all_tied;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) tied += i0 + i < n_cand && sh.list.key[i0 + i] == cut_key;
-    int all_tied;
-    int rank = sh.scan_int.exclusive(tied, all_tied);
-    double sum = 0.;
+    for (int i = 0; i < PER; ++i) tied += tid * PER + i < n_list && sh.key[tid * PER + i] == cut_key;
+    int rank = sh.ints.exclusive(tied, all_tied);
+    if (rank < take && take <= rank + tied) {
+      for (int i = tid * PER; i < n_list; ++i)
+        if (sh.key[i] == cut_key && ++rank == take) {
+          sh.cut_index = sh.index[i];
+          break;
+        }
+    }
+    __syncthreads();
+  };
+  // (cut_index is read behind a barrier)
+  auto kept_weight = [&](float x, uint32_t key, int index) {
+    return key > cut_key || (key == cut_key && index <= sh.cut_index) ? weight_of(x, m, c) : 0.;
+  };
+  auto entry_weight = [&](int i) { return kept_weight(value_of(sh.key[i]), sh.key[i], sh.index[i]); };
+
+  n_list = collect([&](const float (&x)[SEG_LANE], int) {
+    unsigned flags = 0;
+#pragma unroll
+    for (int j = 0; j < SEG_LANE; ++j) flags |= (x[j] >= low ? 1u : 0u) << j;
+    return flags;
+  });
+  if (n_list <= LIST) {  // few candidates: all that follows is in LDS
+    if (use_k && n_list > s.top_k) select_count(s.top_k, n_list);
+    if (use_p) select_mass(s.top_p * row.all_mass);
+    apply_min_p();
+    end_of_ties();
+    double w[PER], sum = 0.;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      w[i] = 0.;
-      if (i0 + i < n_cand) {
-        const uint32_t key = sh.list.key[i0 + i];
-        const bool in = key > cut_key || (key == cut_key && rank < take);
-        rank += key == cut_key;
-        const double e = weight_of(value_of(key), m, s.c);
-        if (in && e >= s.min_p) {
-          w[i] = e;
-          sum += e;
-          atomicMin(&sh.low_key, key);
-        }
-      }
+      w[i] = tid * PER + i < n_list ? entry_weight(tid * PER + i) : 0.;
+      sum += w[i];
     }
-    double z;
-    double cum = sh.scan_f64.exclusive(sum, z);
-    const double target = u * z;
+    double z, cum = sh.row.scan.exclusive(sum, z);
+    const double target = row.u * z;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       cum += w[i];
       if (w[i] > 0.) {
-        if (cum > target) atomicMin(&sh.first, i0 + i);
-        atomicMax(&sh.last, i0 + i);
+        if (cum > target) atomicMin(&sh.row.first, tid * PER + i);
+        atomicMax(&sh.row.last, tid * PER + i);
       }
     }
-    const uint32_t lowest = sh.low_key;
-    rank -= tied;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (i0 + i < n_cand && sh.list.key[i0 + i] == lowest) {
-        if (lowest != cut_key || rank < take) atomicMax(&sh.cut_index, sh.list.index[i0 + i]);
-        rank += lowest == cut_key;
-      }
     __syncthreads();
-    if (tid == 0)
-      finish(sh.list.index[sh.first != 0x7fffffff ? sh.first : sh.last], z, value_of(lowest), sh.cut_index);
+    if (tid == 0) {
+      const int at = sh.row.first != NO_INDEX ? sh.row.first : sh.row.last;
+      row.finish(sh.index[at], z, cut_key == 0 ? low : value_of(cut_key), sh.cut_index);
+    }
     return;
   }
-  // Too many for the list: once over the segments for their ties, once for their masses, the token's once more.
-  // (`list` is not read any more, `seg` takes its place.)
-  __syncthreads();
-  for (int i = wave; i < n_active; i += WAVES) {
-    float x[SEG_LANE];
-    load_seg<E>(x_row, (int)sh.active[i] * SEG, a.V, lane, x);
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j) n += x[j] >= low && key_of(x[j]) == cut_key;
-    n = wave_sum(n);
-    if (lane == 0) sh.seg.ties[i] = n;
-  }
-  __syncthreads();
+
+  // ---- many candidates ----
+  // With one of top-k and top-p: bins over (max - x), with counts or with masses that are approximate from below and above,
+  // tell where the cut can lie; what is above goes into the segments' masses in 64 bits, and only the logits of those bins
+  // into the list, for the exact cut. With both, or many ties of one value: radix selection over the segments.
   const int act_per = (n_active + THREADS - 1) / THREADS;
   const int act_begin = min(tid * act_per, n_active), act_end = min(act_begin + act_per, n_active);
-  {
-    int n = 0, total;
-    for (int i = act_begin; i < act_end; ++i) n += sh.seg.ties[i];
-    int cum = sh.scan_int.exclusive(n, total);
-    for (int i = act_begin; i < act_end; ++i) {
-      const int own_ties = sh.seg.ties[i];
-      sh.seg.ties[i] = cum;
-      cum += own_ties;
-    }
-  }
-  __syncthreads();
-  // weights of the kept logits of active segment i; the lowest key among them and its last index
-  auto kept_weights = [&](int i, double (&w)[SEG_LANE], float (&x)[SEG_LANE]) {
-    load_seg<E>(x_row, (int)sh.active[i] * SEG, a.V, lane, x);
-    unsigned tied = 0;
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j) tied |= (x[j] >= low && key_of(x[j]) == cut_key ? 1u : 0u) << j;
-    int starts[G];
-    order_in_wave<E>(tied, sh.seg.ties[i], starts);
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j) {
-      const uint32_t key = key_of(x[j]);
-      const int rank = starts[j / VEC] + __popc((tied >> (j / VEC * VEC)) & ((1u << (j % VEC)) - 1));
-      const bool in = x[j] >= low && (key > cut_key || (key == cut_key && rank < take));
-      const double e = weight_of(x[j], m, s.c);
-      const bool keep = in && e >= s.min_p;
-      w[j] = keep ? e : 0.;
-      if (!keep) x[j] = pos_inf();
-    }
-  };
-  for (int i = wave; i < n_active; i += WAVES) {
-    double w[SEG_LANE], sum = 0.;
-    float x[SEG_LANE];
-    kept_weights(i, w, x);
-    float lowest = x[0];
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j) {
-      sum += w[j];
-      lowest = fminf(lowest, x[j]);
-    }
-    sum = wave_sum(sum);
-    lowest = wave_min(lowest);
-    if (lane == 0) {
-      sh.seg.mass[i] = sum;
-      if (lowest < pos_inf()) atomicMin(&sh.low_key, key_of(lowest));
-    }
-  }
-  __syncthreads();
-  double own_mass = 0.;
-  for (int i = act_begin; i < act_end; ++i) own_mass += sh.seg.mass[i];
-  double z;
-  const double front = sh.scan_f64.exclusive(own_mass, z);
-  const double target = u * z;
-  double cum = front;
-  for (int i = act_begin; i < act_end; ++i) {
-    const double w = sh.seg.mass[i];
-    if (w > 0.) {
-      if (cum + w > target) {
-        atomicMin(&sh.first, i);
-        break;
+  bool selected = !(use_k && use_p) && c > 1e-20 && c < 1e30 && fabs(m * c) < 1e9;
+  if (selected) {
+    const float rate = (float)c, range = fminf((top - low) * rate, 64.f);  // (what is further down shares the last bin)
+    const float per_binade = range > 0.f ? -(float)BINS / range : 0.f;
+    // in binades below the maximum; falls with x, so that bins are ranges of logits
+    auto depth_of = [&](float x) { return (x - top) * rate; };
+    auto bin_of = [&](float depth) { return min((int)fminf(depth * per_binade, (float)BINS), BINS - 1); };
+    int64_t want = s.top_k;
+    int bin_low = BINS, bin_high = -1;  // nothing is cut off
+    if (use_k || use_p) {
+      for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+      if (tid == 0) {
+        sh.bin_low = BINS - 1;
+        sh.bin_high = BINS - 1;
       }
-      atomicMax(&sh.last, i);
+      __syncthreads();
+      // masses in 2^-32. A depth is off by 3 roundings of 2^-24 of at most 32 binades: 4e-6 of the exponential, whose own
+      // error and truncation, 2^-23 and one unit, come to it
+      sweep([&](const float (&x)[SEG_LANE], int) {
+#pragma unroll
+        for (int j = 0; j < SEG_LANE; ++j)
+          if (x[j] >= low) {
+            const float depth = depth_of(x[j]);
+            const unsigned v = use_k ? 1u : (unsigned)(fast_exp2(depth) * 4294967040.f);
+            atomicAdd(&sh.bins[bin_of(depth)], (unsigned long long)v);
+          }
+      });
+      __syncthreads();
+      constexpr int OWN = BINS / THREADS;
+      unsigned long long own = 0, total;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) own += sh.bins[tid * OWN + i];
+      unsigned long long cum = sh.wide.exclusive(own, total);
+      const double least = use_k ? (double)want : s.top_p * row.all_mass * 4294967296.;
+      const double off = use_k ? 0. : 2e-5 * row.all_mass * 4294967296. + a.V + 512.;
+      const unsigned long long low_mass = (unsigned long long)fmax(ceil(least - off), 0.);
+      const unsigned long long high_mass = (unsigned long long)ceil(least + off);
+      unsigned long long front = 0;
+      int first_low = BINS, first_high = BINS;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const unsigned long long next = cum + sh.bins[tid * OWN + i];
+        if (first_low == BINS && next >= low_mass) {
+          first_low = tid * OWN + i;
+          front = cum;
+        }
+        if (first_high == BINS && next >= high_mass) first_high = tid * OWN + i;
+        cum = next;
+      }
+      if (first_low < BINS) atomicMin(&sh.bin_low, first_low);
+      if (first_high < BINS) atomicMin(&sh.bin_high, first_high);
+      __syncthreads();
+      if (first_low == sh.bin_low) sh.above = front;  // (a count, for top-k)
+      __syncthreads();
+      if (use_k ? total > (unsigned long long)want : total >= low_mass) {
+        bin_low = sh.bin_low;
+        bin_high = sh.bin_high;
+        if (use_k) want -= (int64_t)sh.above;
+      }
     }
-    cum += w;
+    __syncthreads();
+    // the same as limits on the logits: from `sure` on they are in, from `from` on they are in the list
+    auto limit = [&](int bin) {  // the lowest logit of bins up to this one
+      return value_of(first_key([&](uint32_t key) {
+        const float x = value_of(key);
+        return x >= low && bin_of(depth_of(x)) <= bin;
+      }));
+    };
+    const float sure = bin_high < 0 ? low : bin_low > 0 ? limit(bin_low - 1) : pos_inf();
+    const float from = bin_high < 0 ? pos_inf() : limit(bin_high);
+    const float nowhere = (float)fmax(m - 1000. / c, -3.402823466e38);  // 2^-1000 of the maximum, or next to it
+    n_list = collect([&](const float (&x)[SEG_LANE], int i) {
+      unsigned flags = 0;
+      double sum = 0.;
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j) {
+        const bool in = x[j] >= sure;
+        const double z = (double)stat_max(in ? x[j] : nowhere, nowhere) - m, n = fma(z, c, ROUND);
+        sum += exp2_parts(fma(z, c, ROUND - n), n);
+        flags |= (!in && x[j] >= from ? 1u : 0u) << j;
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) sh.seg_mass[i] = sum;
+      return flags;
+    });
+    selected = n_list <= LIST;
+    if (selected) {
+      double own = 0., sure_mass;
+      for (int i = act_begin; i < act_end; ++i) own += sh.seg_mass[i];
+      sh.row.scan.exclusive(own, sure_mass);
+      if (use_k && bin_high >= 0) select_count(want, n_list);
+      if (use_p) select_mass(s.top_p * row.all_mass - sure_mass);
+      end_of_ties();
+      for (int i = act_begin; i < act_end; ++i) {
+        double w = sh.seg_mass[i];
+        const int stop = i + 1 < n_active ? sh.seg_first[i + 1] : n_list;
+        for (int j = sh.seg_first[i]; j < stop; ++j) w += entry_weight(j);
+        sh.seg_mass[i] = w;
+      }
+    }
   }
-  __syncthreads();
-  const int chosen = sh.first != 0x7fffffff ? sh.first : sh.last;
-  if (chosen >= act_begin && chosen < act_end) {
-    double c2 = front;
-    for (int i = act_begin; i < chosen; ++i) c2 += sh.seg.mass[i];
-    sh.target = c2;
-  }
-  const float lowest = value_of(sh.low_key);
-  if (a.kept != nullptr) {  // its last index among the kept
-    for (int i = wave; i < n_active; i += WAVES) {
-      double w[SEG_LANE];
+  if (!selected) {
+    listed = false;
+    if (use_k) {
+      int own = 0, all;
+      each([&](uint32_t) { ++own; });
+      sh.ints.exclusive(own, all);
+      if (all > s.top_k) select_count(s.top_k, all);
+    }
+    if (use_p) select_mass(s.top_p * row.all_mass);
+    apply_min_p();
+    sweep([&](const float (&x)[SEG_LANE], int i) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j) n += x[j] >= low && key_of(x[j]) == cut_key;
+      n = wave_sum(n);
+      if (lane == 0) sh.seg_first[i] = n;
+    });
+    if (tid == 0) sh.bin = -1;
+    __syncthreads();
+    int n = 0, total;
+    for (int i = act_begin; i < act_end; ++i) n += sh.seg_first[i];
+    int cum = sh.ints.exclusive(n, total);
+    for (int i = act_begin; i < act_end; ++i) {
+      if (cum < take && take <= cum + sh.seg_first[i]) {
+        sh.bin = i;
+        sh.ties = take - cum;
+      }
+      cum += sh.seg_first[i];
+    }
+    __syncthreads();
+    if (wave == 0 && sh.bin >= 0) {  // the segment in which the last tie lies
+      const int i = sh.bin;
       float x[SEG_LANE];
-      kept_weights(i, w, x);
-      int last = -1;
+      Raw<E> raw;
+      load_active(i, raw);
+      widen_raw<E>(raw, x);
+      unsigned flags = 0;
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j) flags |= (x[j] >= low && key_of(x[j]) == cut_key ? 1u : 0u) << j;
+      int starts[G];
+      order_in_wave<E>(flags, starts);
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j)
-        if (x[j] == lowest) last = (int)sh.active[i] * SEG + ((j / VEC) * 64 + lane) * VEC + j % VEC;
-      last = wave_reduce(last, [](int p, int q) { return p > q ? p : q; });
-      if (lane == 0 && last >= 0) atomicMax(&sh.cut_index, last);
+        if ((flags >> j & 1) && order_of<E>(flags, starts, j) + 1 == sh.ties)
+          sh.cut_index = (int)sh.active[i] * SEG + place_of<E>(j, lane);
     }
+    __syncthreads();
+    sweep([&](const float (&x)[SEG_LANE], int i) {
+      const int base = (int)sh.active[i] * SEG;
+      double sum = 0.;
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j)
+        if (x[j] >= low) sum += kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane));
+      sum = wave_sum(sum);
+      if (lane == 0) sh.seg_mass[i] = sum;
+    });
   }
   __syncthreads();
+  double own = 0., z;
+  for (int i = act_begin; i < act_end; ++i) own += sh.seg_mass[i];
+  const double front = sh.row.scan.exclusive(own, z);
+  const double target = row.u * z;
+  const int chosen = row.choose(act_begin, act_end, front, target, [&](int i) { return sh.seg_mass[i]; });
   if (wave == 0) {
-    double w[SEG_LANE];
+    const int base = (int)sh.active[chosen] * SEG;
     float x[SEG_LANE];
-    kept_weights(chosen, w, x);
-    const Picked p = wave_pick<E>(w, (int)sh.active[chosen] * SEG, sh.target, target, lane);
-    if (lane == 0) finish(p.index, z, lowest, sh.cut_index);
+    double w[SEG_LANE];
+    Raw<E> raw;
+    load_active(chosen, raw);
+    widen_raw<E>(raw, x);
+#pragma unroll
+    for (int j = 0; j < SEG_LANE; ++j)
+      w[j] = x[j] >= low ? kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane)) : 0.;
+    const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
+    if (lane == 0) row.finish(token, z, cut_key == 0 ? low : value_of(cut_key), sh.cut_index);
   }
 }
 
@@ -805,13 +1054,13 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(Call a, unsigned units
   const int seg = (int)(unit - r * (unsigned)a.segs), base = seg * SEG;
   const float cut = a.cut[r];
   const int cut_index = a.cut_index[r];
-  unsigned flags = 0;  // bit g * VEC + j
-  if (a.seg_max[unit] >= cut) {
+  unsigned flags = 0;  // bit i: element i of the lane
+  if (a.seg_max[unit] >= cut && cut < pos_inf()) {
     float x[SEG_LANE];
     load_seg<E>((const typename E::S*)a.logits + (row0 + r) * a.ld, base, a.V, lane, x);
 #pragma unroll
     for (int i = 0; i < SEG_LANE; ++i) {
-      const int at = base + ((i / VEC) * 64 + lane) * VEC + i % VEC;
+      const int at = base + place_of<E>(i, lane);
       flags |= (x[i] > cut || (x[i] == cut && at <= cut_index) ? 1u : 0u) << i;
     }
   }
@@ -853,11 +1102,31 @@ struct Layout {
 
 template <class E>
 int launch_sample(Call a, int64_t n, const Layout& l, hipStream_t stream) {
+  // no row with a limit, or every row with the smallest
+  const bool whole = (a.temperature_rows == nullptr && a.temperature <= 0.) ||
+                     (a.top_k_rows == nullptr && a.top_p_rows == nullptr && a.min_p_rows == nullptr &&
+                      (a.top_k == 1 || a.top_p <= 0. || ((a.top_k <= 0 || a.top_k >= a.V) && a.top_p >= 1. && a.min_p <= 0.)));
   for (int64_t row0 = 0; row0 < n; row0 += l.rows) {
     const int64_t rows = std::min(l.rows, n - row0);
     const unsigned units = (unsigned)(rows * a.segs), blocks = (units + 3) / 4;
-    hipLaunchKernelGGL((sample_segments_kernel<E, false>), dim3(blocks), dim3(256), 0, stream, a, units, row0);
-    hipLaunchKernelGGL((sample_rows_kernel<E, 1024>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
+    auto segments = [&](auto group) {
+      constexpr int GROUP = decltype(group)::value;
+      const unsigned groups = (unsigned)((a.segs + GROUP - 1) / GROUP), waves = (unsigned)rows * groups;
+      hipLaunchKernelGGL((sample_segments_kernel<E, GROUP>), dim3((waves + 3) / 4), dim3(256), 0, stream, a, waves, groups,
+                         row0);
+    };
+    if (units >= MANY_SEGS)
+      segments(std::integral_constant<int, 4>{});
+    else
+      segments(std::integral_constant<int, 1>{});
+    if (whole)
+      hipLaunchKernelGGL((sample_whole_kernel<E>), dim3((unsigned)rows), dim3(256), 0, stream, a, row0);
+    else if (a.segs > FEW_SEGS)
+      hipLaunchKernelGGL((sample_rows_kernel<E, 1024, MAX_SEGS>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
+    else if (rows > FEW_ROWS)
+      hipLaunchKernelGGL((sample_rows_kernel<E, 512, FEW_SEGS>), dim3((unsigned)rows), dim3(512), 0, stream, a, row0);
+    else
+      hipLaunchKernelGGL((sample_rows_kernel<E, 1024, FEW_SEGS>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
     if (a.kept != nullptr)
       hipLaunchKernelGGL((sample_kept_kernel<E>), dim3(blocks), dim3(256), 0, stream, a, units, row0);
     AREAL_CHECK_LAUNCH();
@@ -870,7 +1139,7 @@ int launch_sample(Call a, int64_t n, const Layout& l, hipStream_t stream) {
 extern "C" {
 
 size_t areal_sample_tokens_workspace_bytes(int64_t N, int64_t V) {
-  if (N <= 0 || V <= 0 || V > MAX_SEGS * SEG) return 0;
+  if (N <= 0 || V <= 0 || V > (int64_t)MAX_SEGS * SEG) return 0;
   return (size_t)Layout(N, V).bytes;
 }
 
@@ -886,7 +1155,7 @@ int areal_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t N, in
     return AREAL_ERR_BAD_ARG;
   if (N == 0) return AREAL_OK;
   if (!logits || !uniforms || !tokens || !logprobs || !full_logprobs) return AREAL_ERR_BAD_ARG;
-  if (V > MAX_SEGS * SEG) return AREAL_ERR_UNSUPPORTED;
+  if (V > (int64_t)MAX_SEGS * SEG) return AREAL_ERR_UNSUPPORTED;
   const Layout l(N, V);
   if (workspace == nullptr || workspace_bytes < (size_t)l.bytes) return AREAL_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return AREAL_ERR_ALIGNMENT;
@@ -894,7 +1163,7 @@ int areal_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t N, in
   Call a{};
   a.logits = logits; a.ld = ld; a.V = (int)V; a.segs = (int)ceil_div_i64(V, SEG);
   a.uniforms = uniforms; a.wide_uniforms = uniforms_fp64 != 0;
-  a.temperature = temperature; a.temperature_rows = temperature_rows;
+  a.temperature = temperature; a.rate = rate_of(temperature); a.temperature_rows = temperature_rows;
   a.top_k = top_k; a.top_k_rows = top_k_rows; a.wide_top_k = top_k_int64 != 0;
   a.top_p = top_p; a.top_p_rows = top_p_rows; a.min_p = min_p; a.min_p_rows = min_p_rows;
   a.subs = top_k_rows != nullptr || (top_k > 1 && top_k < V);
