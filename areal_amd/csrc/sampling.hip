@@ -22,6 +22,7 @@ constexpr int MAX_SEGS = 4096;       // vocabularies up to 4 Mi
 constexpr int FEW_SEGS = 512;        // up to 512 Ki
 constexpr unsigned MANY_SEGS = 16384;  // from here a wave takes four segments of the first pass
 constexpr int64_t FEW_ROWS = 256;
+constexpr int64_t SPREAD_ROWS = 128;   // up to here rows with many candidates are spread over workgroups
 constexpr int LIST = 4096;           // candidates held in LDS
 constexpr double LOG2E = 1.4426950408889634;
 
@@ -72,6 +73,15 @@ struct FP16 {
   static DEVI float one(_Float16 v) { return (float)v; }
 };
 
+// A row that several workgroups work on.
+struct Spread {
+  int state;  // 1: it is one
+  int n_list;
+  float low, top, sure, from;
+  double all_mass;
+  int64_t want;
+};
+
 // Fixed-size view of a call, by value to every kernel. *_rows: one entry a row, or null for the scalar.
 struct Call {
   const void* logits;
@@ -93,6 +103,12 @@ struct Call {
   float* sub_max;
   float* cut;      // [rows]: kept are logits above it,
   int* cut_index;  // and those equal to it up to this index
+  // of rows that are spread over workgroups (null: none are)
+  Spread* spread;
+  unsigned long long* part_bins;
+  double* part_mass;
+  int2* part_runs;
+  uint2* part_list;
 };
 
 // A row's settings. top_k: V where there is no limit; top1: the first of the order alone.
@@ -367,17 +383,20 @@ struct Row {
   float top;
   double m, u, all_mass, before;
 
-  DEVI Row(const Call& call, RowShared<THREADS>& shared, int64_t row0)
-      : a(call), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), r(blockIdx.x),
-        row(row0 + blockIdx.x), x_row((const typename E::S*)a.logits + row * a.ld),
+  DEVI Row(const Call& call, RowShared<THREADS>& shared, int64_t row0, unsigned row_in_launch)
+      : a(call), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), r(row_in_launch),
+        row(row0 + row_in_launch), x_row((const typename E::S*)a.logits + row * a.ld),
         seg_max(a.seg_max + (int64_t)r * a.segs), seg_sum(a.seg_sum + (int64_t)r * a.segs), s(settings_of(a, row)) {}
 
   DEVI double seg_mass(int i) const { return seg_sum[i] * weight_of(seg_max[i], m, s.c); }
 
+  DEVI double uniform() const {
+    const double v = a.wide_uniforms ? ((const double*)a.uniforms)[row] : (double)((const float*)a.uniforms)[row];
+    return fmin(fmax(v, 0.), 1.);
+  }
   // Largest logit and mass of the row. False: there is no distribution (and the outputs say so).
   DEVI bool combine() {
-    u = a.wide_uniforms ? ((const double*)a.uniforms)[row] : (double)((const float*)a.uniforms)[row];
-    u = fmin(fmax(u, 0.), 1.);
+    u = uniform();
     const int per = (a.segs + THREADS - 1) / THREADS;
     begin = min(tid * per, a.segs);
     end = min(begin + per, a.segs);
@@ -493,11 +512,13 @@ struct Row {
 template <class E>
 __global__ __launch_bounds__(256) void sample_whole_kernel(Call a, int64_t row0) {
   __shared__ RowShared<256> sh;
-  Row<E, 256> row(a, sh, row0);
+  Row<E, 256> row(a, sh, row0, blockIdx.x);
   if (row.combine()) row.simple();
 }
 
 constexpr int BINS = 2048;
+constexpr int PART = 16;  // segments of a workgroup where a row is spread over several: one per wave
+
 template <int THREADS, int SEGS>
 struct CutShared {
   static constexpr int WAVES = THREADS / 64;
@@ -509,62 +530,73 @@ struct CutShared {
     uint32_t count[256];
   };
   unsigned long long above;
-  int bin, ties, bin_low, bin_high, cut_index;
-  int wave_count[2][WAVES];
-  unsigned short active[SEGS];
-  int seg_first[SEGS];  // of an active segment: entries of the list before its own, or ties
-  uint32_t key[LIST];   // the list, in index order
-  int index[LIST];
+  int bin, ties, bin_low, bin_high, cut_index, n_list;
+  float limits[2];
+  unsigned short active[SEGS];  // segments that reach the lower bound
+  int seg_first[SEGS], seg_count[SEGS];  // their entries of the list: a run of it each, in index order
   union {
     unsigned long long bins[BINS];
     double seg_mass[SEGS];
   };
+  uint2 entry[LIST];  // .x: key, later the entry's weight in its place
+  int index[LIST];
 };
 
-// The others. The kept set is a prefix of the order: it ends at a key (`cut_key`) and at an index among that key's ties.
+// A row whose kept set is a proper prefix of the order: the set ends at a key (`cut_key`) and at an index among that key's
+// ties. THREADS threads work on it, or the workgroups of several launches.
 template <class E, int THREADS, int SEGS>
-__global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t row0) {
-  constexpr int VEC = E::VEC, G = SEG_LANE / VEC, WAVES = THREADS / 64, LOW = E::LOW;
-  __shared__ CutShared<THREADS, SEGS> sh;
-  Row<E, THREADS> row(a, sh.row, row0);
-  if (!row.combine() || row.simple()) return;
-  const Settings& s = row.s;
-  const int tid = row.tid, lane = row.lane, wave = row.wave;
-  const double m = row.m, c = s.c;
-  const float top = row.top;
-  const bool use_k = s.top_k < a.V, use_p = s.top_p < 1., use_min = s.min_p > 0.;
-  const uint32_t top_key = key_of(top);
-  if (tid == 0) sh.cut_index = NO_INDEX;
+struct Cut : Row<E, THREADS> {
+  static constexpr int VEC = E::VEC, G = SEG_LANE / VEC, WAVES = THREADS / 64, LOW = E::LOW;
+  using Base = Row<E, THREADS>;
+  using Base::a; using Base::tid; using Base::lane; using Base::wave; using Base::r; using Base::s; using Base::m;
+  using Base::top; using Base::all_mass; using Base::x_row; using Base::seg_max; using Base::u;
+  CutShared<THREADS, SEGS>& sh;
+  bool use_k, use_p, min_last;  // min_last: min_p counts behind the others
+  uint32_t top_key, min_key = 0, cut_key = 0;
+  int take = NO_INDEX;              // of the ties of cut_key, by index
+  unsigned long long tied_out = 0;  // mass of those that top-k leaves out
+  float low;                        // no kept logit is below
+  int n_active = 0, n_list = 0, begin_active = 0, end_active = 0;
+  bool listed = true;
+  // bits in which keys from `low` on can differ: those below top_bits, and not the type's own lowest
+  int top_bits;
+  uint32_t common;
+
+  DEVI Cut(const Call& call, CutShared<THREADS, SEGS>& shared, int64_t row0, unsigned row_in_launch)
+      : Base(call, shared.row, row0, row_in_launch), sh(shared) {
+    use_k = s.top_k < a.V;
+    use_p = s.top_p < 1.;
+    min_last = use_k && use_p && s.min_p > 0.;
+  }
+
   // The first key from 0 to top_key for which `reached` holds, which it does from some key on (and at top_key): 64 probes
-  // a round, by every wave for itself.
-  auto first_key = [&](auto reached) {
+  // a round.
+  template <class F>
+  DEVI uint32_t first_key(F reached) const {
     uint32_t from = 0, to = top_key;  // the answer lies in [from, to]
     while (from < to) {
       const uint32_t step = (to - from) / 64 + 1;
       const uint64_t probe64 = (uint64_t)from + (uint64_t)step * lane;
       const uint32_t probe = probe64 < to ? (uint32_t)probe64 : to;
       const unsigned long long hit = __builtin_amdgcn_ballot_w64(reached(probe));
-      const int at = __builtin_ctzll(hit | 1ull << 63);  // (the last probe is reached or below the answer by a step at most)
-      const bool any = hit != 0;
-      const uint32_t found = __builtin_amdgcn_readlane(probe, at);
-      if (!any) {
-        from = found + 1;
+      if (hit == 0) {  // behind the last probe
+        from = __builtin_amdgcn_readlane(probe, 63) + 1;
       } else {
-        const uint32_t before = at == 0 ? from : __builtin_amdgcn_readlane(probe, at - 1) + 1;
-        from = before;
-        to = found;
+        const int at = __builtin_ctzll(hit);
+        to = __builtin_amdgcn_readlane(probe, at);
+        if (at > 0) from = __builtin_amdgcn_readlane(probe, at - 1) + 1;
       }
     }
     return to;
-  };
+  }
 
-  auto clear_bins = [&] {  // 256 of them
+  DEVI void clear_bins() {  // 256 of them
     __syncthreads();
     for (int i = tid; i < 256; i += THREADS) sh.mass[i] = 0;
     __syncthreads();
-  };
-  // the bin, from the 256th downwards, in which the running count reaches `want`: sh.bin, the count in front and its own
-  auto find_count = [&](int64_t want) {
+  }
+  // The bin, from the 256th downwards, in which the running count reaches `want`: sh.bin, the count in front and its own.
+  DEVI void find_count(int64_t want) {
     __syncthreads();
     if (wave == 0) {
       uint32_t n4[4];
@@ -588,58 +620,77 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       }
     }
     __syncthreads();
-  };
-
-  // ---- a lower bound on the kept logits, so that few are looked at ----
-  double bound = -1.7e308;
-  // No token lighter than this is in S2: all those together weigh less than (1 - top_p) of the mass.
-  if (use_p && !use_k) bound = fmax(bound, m + log2((1. - s.top_p) * row.all_mass / a.V) / c);
-  bound -= 1e-6 * fabs(bound) + 1e-6 / c;
-  float low = bound > -3.4e38 ? (float)bound : -3.402823466e38f;
-  // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
-  const uint32_t min_key =
-      use_min ? first_key([&](uint32_t key) {
-        const float x = value_of(key);
-        return x == x && weight_of(x, m, c) >= s.min_p;  // (the lowest keys are NaN's, and -inf's)
-      })
-              : 0;
-  const bool min_last = use_k && use_p;
-  if (use_min && !min_last) low = fmaxf(low, value_of(min_key));
-  if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
-    // top_k maxima of disjoint parts of the row are that many logits: the top_k-th largest of the row is no lower than
-    // theirs. Its upper 16 bits are enough.
-    const float* subs = a.sub_max + (int64_t)row.r * a.segs * SUBS;
-    const int n = a.segs * SUBS;
-    uint32_t prefix = 0;
-    int64_t want = s.top_k;
-#pragma unroll
-    for (int shift = 24; shift >= 16; shift -= 8) {
-      clear_bins();
-      for (int i = tid; i < n; i += THREADS) {
-        const uint32_t key = key_of(subs[i]);
-        if (shift == 24 || (key >> 24) == (prefix >> 24)) atomicAdd(&sh.count[(key >> shift) & 255], 1u);
-      }
-      find_count(want);
-      prefix |= (uint32_t)sh.bin << shift;
-      want -= (int64_t)sh.above;
-    }
-    const float lowest = value_of(prefix);
-    if (lowest > low) low = lowest;  // (not where it is a NaN's pattern, below that of -inf)
   }
 
-  // ---- the segments that reach it, in index order ----
-  int n_active;
-  {
+  DEVI void range_of_keys() {
+    const uint32_t low_key = key_of(low);
+    top_bits = low_key == top_key ? 0 : 32 - __builtin_clz(low_key ^ top_key);
+    common = top_bits == 32 ? 0 : ~0u << top_bits;
+  }
+
+  // A lower bound on the kept logits, so that few are looked at; the segments that reach it, in index order.
+  DEVI void bound() {
+    top_key = key_of(top);
+    low = -3.402823466e38f;
+    if (use_p && !use_k) {
+      // No token lighter than this is in S2: all those together weigh less than (1 - top_p) of the mass.
+      double b = m + log2((1. - s.top_p) * all_mass / a.V) / s.c;
+      b -= 1e-6 * fabs(b) + 1e-6 / s.c;
+      if (b > -3.4e38) low = (float)b;
+    }
+    // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
+    if (s.min_p > 0.) {
+      min_key = first_key([&](uint32_t key) {
+        const float x = value_of(key);
+        return x == x && weight_of(x, m, s.c) >= s.min_p;  // (the lowest keys are NaN's, and -inf's)
+      });
+      if (!min_last) low = fmaxf(low, value_of(min_key));
+    }
+    if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
+      // top_k maxima of disjoint parts of the row are that many logits: the top_k-th largest of the row is no lower than
+      // theirs. Its upper 16 bits are enough.
+      const float* subs = a.sub_max + (int64_t)r * a.segs * SUBS;
+      const int n = a.segs * SUBS;
+      uint32_t prefix = 0;
+      int64_t want = s.top_k;
+#pragma unroll
+      for (int shift = 24; shift >= 16; shift -= 8) {
+        clear_bins();
+        for (int i = tid; i < n; i += THREADS) {
+          const uint32_t key = key_of(subs[i]);
+          if (shift == 24 || (key >> 24) == (prefix >> 24)) atomicAdd(&sh.count[(key >> shift) & 255], 1u);
+        }
+        find_count(want);
+        prefix |= (uint32_t)sh.bin << shift;
+        want -= (int64_t)sh.above;
+      }
+      const float lowest = value_of(prefix);
+      if (lowest > low) low = lowest;  // (not where it is a NaN's pattern, below that of -inf)
+    }
+    range_of_keys();
     int mine = 0;
-    for (int i = row.begin; i < row.end; ++i) mine += row.seg_max[i] >= low;
+    for (int i = Base::begin; i < Base::end; ++i) mine += seg_max[i] >= low;
     int at = sh.ints.exclusive(mine, n_active);
-    for (int i = row.begin; i < row.end; ++i)
-      if (row.seg_max[i] >= low) sh.active[at++] = (unsigned short)i;
+    for (int i = Base::begin; i < Base::end; ++i)
+      if (seg_max[i] >= low) sh.active[at++] = (unsigned short)i;
+    share_active();
+  }
+  DEVI void share_active() {
+    const int per = (n_active + THREADS - 1) / THREADS;
+    begin_active = min(tid * per, n_active);
+    end_active = min(begin_active + per, n_active);
+    if (tid == 0) {
+      sh.cut_index = NO_INDEX;
+      sh.n_list = 0;
+    }
     __syncthreads();
   }
-  auto load_active = [&](int i, Raw<E>& x) { load_raw<E>(row.x_row, (int)sh.active[i] * SEG, a.V, lane, x); };
+
+  DEVI int base_of(int i) const { return (int)sh.active[i] * SEG; }
+  DEVI void load_active(int i, Raw<E>& x) const { load_raw<E>(x_row, base_of(i), a.V, lane, x); }
   // f(logits, i) of active segment i, a wave each; the next one's loads are under way meanwhile
-  auto sweep = [&](auto f) {
+  template <class F>
+  DEVI void sweep(F f) {
     Raw<E> now, next;
     if (wave < n_active) load_active(wave, now);
     for (int i = wave; i < n_active; i += WAVES) {
@@ -649,55 +700,48 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       f(x, i);
       now = next;
     }
-  };
-  // Puts the logits that flags_of(logits, i) marks into the list, in index order, and the number of them in front of each
-  // active segment into seg_first. Returns their number; one of more than LIST as soon as it is.
-  auto collect = [&](auto flags_of) {
-    int n = 0;
-    Raw<E> now, next;
-    if (wave < n_active) load_active(wave, now);
-    for (int i0 = 0, half = 0; i0 < n_active; i0 += WAVES, half ^= 1) {
-      const int i = i0 + wave;
-      float x[SEG_LANE];
-      unsigned flags = 0;
-      if (i + WAVES < n_active) load_active(i + WAVES, next);
-      widen_raw<E>(now, x);
-      if (i < n_active) flags = flags_of(x, i);
+  }
+  // Appends the logits marked by `flags` (bit j: element j of the lane) to a list, in index order from entry `to` on.
+  DEVI void append(const float (&x)[SEG_LANE], unsigned flags, const int (&starts)[G], int to, int base, uint2* entry,
+                   int* index) const {
+#pragma unroll
+    for (int j = 0; j < SEG_LANE; ++j) {
+      const int p = to + order_of<E>(flags, starts, j);
+      if ((flags >> j & 1) && p < LIST) {
+        const int at = base + place_of<E>(j, lane);
+        entry[p].x = key_of(x[j]);
+        if (index != nullptr) index[p] = at;
+        else entry[p].y = (uint32_t)at;
+      }
+    }
+  }
+  // The logits that flags_of(logits, i) marks, as the list; segments take runs of it in any order. Once they are too many
+  // for it, segments are left out.
+  template <class F>
+  DEVI void collect(F flags_of) {
+    sweep([&](const float (&x)[SEG_LANE], int i) {
+      if (*(volatile int*)&sh.n_list > LIST) return;
+      const unsigned flags = flags_of(x, i);
       int starts[G];
       const int own = order_in_wave<E>(flags, starts);
-      if (lane == 0) sh.wave_count[half][wave] = own;
-      __syncthreads();  // (the other half's readers are behind the next one)
-      int to = n;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) to += sh.wave_count[half][w];
-        n += sh.wave_count[half][w];
+      int to = 0;
+      if (lane == 0) {
+        to = atomicAdd(&sh.n_list, own);
+        sh.seg_first[i] = to;
+        sh.seg_count[i] = own;
       }
-      if (lane == 0 && i < n_active) sh.seg_first[i] = to;
-      if (flags != 0) {
-        const int base = (int)sh.active[i] * SEG;
-#pragma unroll
-        for (int j = 0; j < SEG_LANE; ++j) {
-          const int p = to + order_of<E>(flags, starts, j);
-          if ((flags >> j & 1) && p < LIST) {
-            sh.key[p] = key_of(x[j]);
-            sh.index[p] = base + place_of<E>(j, lane);
-          }
-        }
-      }
-      if (n > LIST) break;
-      now = next;
-    }
+      to = __builtin_amdgcn_readfirstlane(to);
+      if (flags != 0) append(x, flags, starts, to, base_of(i), sh.entry, sh.index);
+    });
     __syncthreads();
-    return n;
-  };
+    n_list = sh.n_list;
+  }
 
   // ---- selection among candidates: the list, or the active segments' logits from `low` on ----
-  bool listed = true;
-  int n_list = 0;
-  auto each = [&](auto f) {  // f(key), in any order
+  template <class F>
+  DEVI void each(F f) {  // f(key), in any order
     if (listed) {
-      for (int i = tid; i < n_list; i += THREADS) f(sh.key[i]);
+      for (int i = tid; i < n_list; i += THREADS) f(sh.entry[i].x);
     } else {
       sweep([&](const float (&x)[SEG_LANE], int) {
 #pragma unroll
@@ -705,30 +749,24 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
           if (x[j] >= low) f(key_of(x[j]));
       });
     }
-  };
-  // Bits in which candidates' keys can differ: those below `top_bits`, and not the type's own lowest.
-  const uint32_t low_key = key_of(low);
-  const int top_bits = low_key == top_key ? 0 : 32 - __builtin_clz(low_key ^ top_key);
-  const uint32_t common = top_bits == 32 ? 0 : ~0u << top_bits;
-  auto whole_key = [&](uint32_t prefix) { return prefix | ((prefix >> 31) ? 0u : (1u << LOW) - 1); };
-
-  uint32_t cut_key = 0;  // kept: keys above it, and of its ties the first `take`
-  int take = NO_INDEX;
-  unsigned long long tied_out = 0;  // mass of the ties of cut_key that top-k leaves out
-  const double unit = (double)(1ull << a.fixed_bits);
-  auto fixed_mass = [&](uint32_t key) {  // 2^52 plus it has it in the low bits, rounded
-    const double w = fma(weight_of(value_of(key), m, c), unit, 4503599627370496.);
+  }
+  DEVI uint32_t whole_key(uint32_t prefix) const { return prefix | ((prefix >> 31) ? 0u : (1u << LOW) - 1); }
+  DEVI double unit() const { return (double)(1ull << a.fixed_bits); }
+  DEVI unsigned long long fixed_mass(uint32_t key) const {  // 2^52 plus it has it in the low bits, rounded
+    const double w = fma(weight_of(value_of(key), m, s.c), unit(), 4503599627370496.);
     return __builtin_bit_cast(unsigned long long, w) & 0xfffffffffffffull;
-  };
-  // The key of the want-th largest candidate.
-  auto select_count = [&](int64_t want, int n) {
+  }
+  // The key of the want-th largest candidate (of which there are more).
+  DEVI void select_count(int64_t want) {
     uint32_t mask = common, prefix = top_key & common;
-    int ties = n;
-    for (int bits = top_bits; bits > LOW;) {
+    int ties = 0;
+    int bits = top_bits;
+    do {
       const int shift = max(bits - 8, LOW);
+      const uint32_t field = (1u << (max(bits, shift) - shift)) - 1;
       clear_bins();
       each([&](uint32_t key) {
-        if ((key & mask) == prefix) atomicAdd(&sh.count[(key >> shift) & ((1u << (bits - shift)) - 1)], 1u);
+        if ((key & mask) == prefix) atomicAdd(&sh.count[(key >> shift) & field], 1u);
       });
       find_count(want);
       prefix |= (uint32_t)sh.bin << shift;
@@ -736,13 +774,13 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       want -= (int64_t)sh.above;
       ties = sh.ties;
       bits = shift;
-    }
+    } while (bits > LOW);
     cut_key = whole_key(prefix);
     take = (int)want;
     tied_out = (unsigned long long)(ties - take) * fixed_mass(cut_key);
-  };
-  // The key at which the candidates' mass reaches `least` (0: top_p of S1's), within S1.
-  auto select_mass = [&](double least) {
+  }
+  // The key at which the candidates' mass reaches `least` (with top-k: top_p of S1's), within S1.
+  DEVI void select_mass(double least) {
     uint32_t mask = common, prefix = top_key & common;
     unsigned long long want = 0;
     int bits = top_bits;
@@ -762,8 +800,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
         const unsigned long long incl =
             wave_inclusive_scan(n, 0ull, [](unsigned long long x, unsigned long long y) { return x + y; });
         if (first) {  // in S2: what has less than this in front of it
-          const double least_fixed =
-              use_k ? s.top_p * (double)(lane_value(incl, 63) - tied_out) : least * unit;
+          const double least_fixed = use_k ? s.top_p * (double)(lane_value(incl, 63) - tied_out) : least * unit();
           want = least_fixed > 1. ? (unsigned long long)ceil(least_fixed) : 1;
         }
         if (lane == 0) sh.bin = -1;
@@ -794,208 +831,225 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
     const int ties = w == 0 ? NO_INDEX : (int)min((want + w - 1) / w, (unsigned long long)NO_INDEX);
     take = key == cut_key ? min(take, ties) : ties;
     cut_key = key;
-  };
-  auto apply_min_p = [&] {
+  }
+  DEVI void apply_min_p() {
     if (min_last && min_key > cut_key) {
       cut_key = min_key;
       take = NO_INDEX;
     }
-  };
-  constexpr int PER = LIST / THREADS;  // list entries of a thread, in order
-  // sh.cut_index: where the first `take` ties of cut_key in the list end
-  auto end_of_ties = [&] {
-    int tied = 0, all_tied;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) tied += tid * PER + i < n_list && sh.key[tid * PER + i] == cut_key;
-    int rank = sh.ints.exclusive(tied, all_tied);
-    if (rank < take && take <= rank + tied) {
-      for (int i = tid * PER; i < n_list; ++i)
-        if (sh.key[i] == cut_key && ++rank == take) {
-          sh.cut_index = sh.index[i];
-          break;
+  }
+  // The active segment in which the take-th tie lies, and which of its ties it is: sh.bin (-1: take has no end), sh.ties.
+  // `ties`: a thread's segments' numbers of them.
+  template <class F>
+  DEVI void find_last_tie(F ties) {
+    __syncthreads();  // (a selection's readers of sh.bin)
+    if (tid == 0) sh.bin = -1;
+    int own = 0, total;
+    if (take != NO_INDEX)
+      for (int i = begin_active; i < end_active; ++i) own += ties(i);
+    int cum = sh.ints.exclusive(own, total);  // (a barrier in front of the writes below)
+    if (take != NO_INDEX && cum < take && take <= cum + own)
+      for (int i = begin_active; i < end_active; ++i) {
+        const int n = ties(i);
+        if (cum < take && take <= cum + n) {
+          sh.bin = i;
+          sh.ties = take - cum;
         }
-    }
-    __syncthreads();
-  };
-  // (cut_index is read behind a barrier)
-  auto kept_weight = [&](float x, uint32_t key, int index) {
-    return key > cut_key || (key == cut_key && index <= sh.cut_index) ? weight_of(x, m, c) : 0.;
-  };
-  auto entry_weight = [&](int i) { return kept_weight(value_of(sh.key[i]), sh.key[i], sh.index[i]); };
-
-  n_list = collect([&](const float (&x)[SEG_LANE], int) {
-    unsigned flags = 0;
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j) flags |= (x[j] >= low ? 1u : 0u) << j;
-    return flags;
-  });
-  if (n_list <= LIST) {  // few candidates: all that follows is in LDS
-    if (use_k && n_list > s.top_k) select_count(s.top_k, n_list);
-    if (use_p) select_mass(s.top_p * row.all_mass);
-    apply_min_p();
-    end_of_ties();
-    double w[PER], sum = 0.;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      w[i] = tid * PER + i < n_list ? entry_weight(tid * PER + i) : 0.;
-      sum += w[i];
-    }
-    double z, cum = sh.row.scan.exclusive(sum, z);
-    const double target = row.u * z;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      cum += w[i];
-      if (w[i] > 0.) {
-        if (cum > target) atomicMin(&sh.row.first, tid * PER + i);
-        atomicMax(&sh.row.last, tid * PER + i);
+        cum += n;
       }
+    __syncthreads();
+  }
+  // (cut_index is read behind a barrier)
+  DEVI double kept_weight(float x, uint32_t key, int at) const {
+    return key > cut_key || (key == cut_key && at <= sh.cut_index) ? weight_of(x, m, s.c) : 0.;
+  }
+  // The list's part of the kept set: weights in place of keys, added to the segments' masses.
+  DEVI void weigh_list() {
+    auto ties = [&](int i) {
+      int n = 0;
+      for (int j = sh.seg_first[i]; j < sh.seg_first[i] + sh.seg_count[i]; ++j) n += sh.entry[j].x == cut_key;
+      return n;
+    };
+    if (take != NO_INDEX) {
+      find_last_tie(ties);
+      if (sh.bin >= begin_active && sh.bin < end_active) {
+        int rank = 0, j = sh.seg_first[sh.bin];
+        while ((rank += sh.entry[j].x == cut_key) < sh.ties) ++j;
+        sh.cut_index = sh.index[j];
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < n_list; i += THREADS) {
+      const uint32_t key = sh.entry[i].x;
+      sh.entry[i] = __builtin_bit_cast(uint2, kept_weight(value_of(key), key, sh.index[i]));
     }
     __syncthreads();
-    if (tid == 0) {
-      const int at = sh.row.first != NO_INDEX ? sh.row.first : sh.row.last;
-      row.finish(sh.index[at], z, cut_key == 0 ? low : value_of(cut_key), sh.cut_index);
-    }
-    return;
+  }
+  DEVI double list_mass(int i) const {
+    double w = 0.;
+    for (int j = sh.seg_first[i]; j < sh.seg_first[i] + sh.seg_count[i]; ++j) w += __builtin_bit_cast(double, sh.entry[j]);
+    return w;
+  }
+  DEVI void finish_cut(int token, double z) const {
+    // without a selection all from `low` on are kept
+    Base::finish(token, z, cut_key == 0 ? low : value_of(cut_key), sh.cut_index);
   }
 
-  // ---- many candidates ----
-  // With one of top-k and top-p: bins over (max - x), with counts or with masses that are approximate from below and above,
-  // tell where the cut can lie; what is above goes into the segments' masses in 64 bits, and only the logits of those bins
-  // into the list, for the exact cut. With both, or many ties of one value: radix selection over the segments.
-  const int act_per = (n_active + THREADS - 1) / THREADS;
-  const int act_begin = min(tid * act_per, n_active), act_end = min(act_begin + act_per, n_active);
-  bool selected = !(use_k && use_p) && c > 1e-20 && c < 1e30 && fabs(m * c) < 1e9;
-  if (selected) {
-    const float rate = (float)c, range = fminf((top - low) * rate, 64.f);  // (what is further down shares the last bin)
-    const float per_binade = range > 0.f ? -(float)BINS / range : 0.f;
-    // in binades below the maximum; falls with x, so that bins are ranges of logits
-    auto depth_of = [&](float x) { return (x - top) * rate; };
-    auto bin_of = [&](float depth) { return min((int)fminf(depth * per_binade, (float)BINS), BINS - 1); };
-    int64_t want = s.top_k;
-    int bin_low = BINS, bin_high = -1;  // nothing is cut off
-    if (use_k || use_p) {
-      for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
-      if (tid == 0) {
-        sh.bin_low = BINS - 1;
-        sh.bin_high = BINS - 1;
-      }
-      __syncthreads();
-      // masses in 2^-32. A depth is off by 3 roundings of 2^-24 of at most 32 binades: 4e-6 of the exponential, whose own
-      // error and truncation, 2^-23 and one unit, come to it
-      sweep([&](const float (&x)[SEG_LANE], int) {
-#pragma unroll
-        for (int j = 0; j < SEG_LANE; ++j)
-          if (x[j] >= low) {
-            const float depth = depth_of(x[j]);
-            const unsigned v = use_k ? 1u : (unsigned)(fast_exp2(depth) * 4294967040.f);
-            atomicAdd(&sh.bins[bin_of(depth)], (unsigned long long)v);
-          }
-      });
-      __syncthreads();
-      constexpr int OWN = BINS / THREADS;
-      unsigned long long own = 0, total;
-#pragma unroll
-      for (int i = 0; i < OWN; ++i) own += sh.bins[tid * OWN + i];
-      unsigned long long cum = sh.wide.exclusive(own, total);
-      const double least = use_k ? (double)want : s.top_p * row.all_mass * 4294967296.;
-      const double off = use_k ? 0. : 2e-5 * row.all_mass * 4294967296. + a.V + 512.;
-      const unsigned long long low_mass = (unsigned long long)fmax(ceil(least - off), 0.);
-      const unsigned long long high_mass = (unsigned long long)ceil(least + off);
-      unsigned long long front = 0;
-      int first_low = BINS, first_high = BINS;
-#pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const unsigned long long next = cum + sh.bins[tid * OWN + i];
-        if (first_low == BINS && next >= low_mass) {
-          first_low = tid * OWN + i;
-          front = cum;
-        }
-        if (first_high == BINS && next >= high_mass) first_high = tid * OWN + i;
-        cum = next;
-      }
-      if (first_low < BINS) atomicMin(&sh.bin_low, first_low);
-      if (first_high < BINS) atomicMin(&sh.bin_high, first_high);
-      __syncthreads();
-      if (first_low == sh.bin_low) sh.above = front;  // (a count, for top-k)
-      __syncthreads();
-      if (use_k ? total > (unsigned long long)want : total >= low_mass) {
-        bin_low = sh.bin_low;
-        bin_high = sh.bin_high;
-        if (use_k) want -= (int64_t)sh.above;
-      }
+  // All candidates are in the list.
+  DEVI void few() {
+    if (use_k && n_list > s.top_k) select_count(s.top_k);
+    if (use_p) select_mass(s.top_p * all_mass);
+    apply_min_p();
+    weigh_list();
+    double own = 0., z;
+    for (int i = begin_active; i < end_active; ++i) {
+      const double w = list_mass(i);
+      sh.seg_mass[i] = w;
+      own += w;
     }
+    const double front = sh.row.scan.exclusive(own, z), target = u * z;
+    const int chosen = Base::choose(begin_active, end_active, front, target, [&](int i) { return sh.seg_mass[i]; });
+    if (chosen >= begin_active && chosen < end_active) {
+      double cum = sh.row.target;
+      int token = -1;
+      for (int j = sh.seg_first[chosen]; j < sh.seg_first[chosen] + sh.seg_count[chosen]; ++j) {
+        const double w = __builtin_bit_cast(double, sh.entry[j]);
+        cum += w;
+        if (w > 0.) {
+          token = sh.index[j];
+          if (cum > target) break;
+        }
+      }
+      finish_cut(token, z);
+    }
+  }
+
+  // ---- many candidates, one of top-k and top-p (or only min_p) ----
+  // Bins over (max - x), with counts or with masses that are approximate from below and above, tell where the cut can lie.
+  // What is above goes into the segments' masses in 64 bits, and only the logits of those bins into the list, for the exact
+  // cut. (Not where depths are out of fp32's range.)
+  DEVI bool can_bin() const { return !(use_k && use_p) && s.c > 1e-20 && s.c < 1e30 && fabs(m * s.c) < 1e9; }
+  float rate, per_binade;
+  DEVI void prepare_bins() {
+    rate = (float)s.c;
+    const float range = fminf((top - low) * rate, 64.f);  // (what is further down shares the last bin)
+    per_binade = range > 0.f ? -(float)BINS / range : 0.f;
+  }
+  // binades below the maximum; falls with x, so that bins are ranges of logits
+  DEVI float depth_of(float x) const { return (x - top) * rate; }
+  DEVI int bin_of(float depth) const { return min((int)fminf(depth * per_binade, (float)BINS), BINS - 1); }
+  // Masses in 2^-32. A depth is off by 3 roundings of 2^-24 of at most 32 binades: 4e-6 of the exponential, whose own error
+  // and truncation, 2^-23 and one unit, come to it.
+  DEVI void fill_bins() {
+    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
     __syncthreads();
-    // the same as limits on the logits: from `sure` on they are in, from `from` on they are in the list
-    auto limit = [&](int bin) {  // the lowest logit of bins up to this one
-      return value_of(first_key([&](uint32_t key) {
+    sweep([&](const float (&x)[SEG_LANE], int) {
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j)
+        if (x[j] >= low) {
+          const float depth = depth_of(x[j]);
+          const unsigned v = use_k ? 1u : (unsigned)(fast_exp2(depth) * 4294967040.f);
+          atomicAdd(&sh.bins[bin_of(depth)], (unsigned long long)v);
+        }
+    });
+    __syncthreads();
+  }
+  // From the row's bins, `own` consecutive ones of a thread: logits from `sure` on are kept, and of those from `from` on the
+  // cut takes some; want: how many of these top-k takes (NO_INDEX: there is no cut).
+  static constexpr int OWN = BINS / THREADS;
+  DEVI void bracket(const unsigned long long (&h)[OWN], float& sure, float& from, int64_t& want) {
+    if (tid == 0) sh.bin_low = sh.bin_high = BINS - 1;
+    unsigned long long own = 0, total;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) own += h[i];
+    unsigned long long cum = sh.wide.exclusive(own, total);  // (a barrier behind the line above)
+    const double least = use_k ? (double)s.top_k : s.top_p * all_mass * 4294967296.;
+    const double off = use_k ? 0. : 2e-5 * all_mass * 4294967296. + a.V + 512.;
+    const unsigned long long low_mass = (unsigned long long)fmax(ceil(least - off), 0.);
+    const unsigned long long high_mass = (unsigned long long)ceil(least + off);
+    unsigned long long front = 0;
+    int first_low = BINS, first_high = BINS;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const unsigned long long next = cum + h[i];
+      if (first_low == BINS && next >= low_mass) {
+        first_low = tid * OWN + i;
+        front = cum;
+      }
+      if (first_high == BINS && next >= high_mass) first_high = tid * OWN + i;
+      cum = next;
+    }
+    if (first_low < BINS) atomicMin(&sh.bin_low, first_low);
+    if (first_high < BINS) atomicMin(&sh.bin_high, first_high);
+    __syncthreads();
+    if (first_low == sh.bin_low) sh.above = front;  // (a count, for top-k)
+    want = NO_INDEX;
+    sure = low;
+    from = pos_inf();
+    const bool cut = use_k ? total > (unsigned long long)s.top_k : total >= low_mass;
+    if (!cut) return;
+    // the bins' limits as logits: the lowest of bins up to one
+    if (wave < 2) {
+      const int bin = wave == 0 ? sh.bin_low - 1 : sh.bin_high;
+      const float limit = bin < 0 ? pos_inf() : value_of(first_key([&](uint32_t key) {
         const float x = value_of(key);
         return x >= low && bin_of(depth_of(x)) <= bin;
       }));
-    };
-    const float sure = bin_high < 0 ? low : bin_low > 0 ? limit(bin_low - 1) : pos_inf();
-    const float from = bin_high < 0 ? pos_inf() : limit(bin_high);
-    const float nowhere = (float)fmax(m - 1000. / c, -3.402823466e38);  // 2^-1000 of the maximum, or next to it
-    n_list = collect([&](const float (&x)[SEG_LANE], int i) {
-      unsigned flags = 0;
-      double sum = 0.;
-#pragma unroll
-      for (int j = 0; j < SEG_LANE; ++j) {
-        const bool in = x[j] >= sure;
-        const double z = (double)stat_max(in ? x[j] : nowhere, nowhere) - m, n = fma(z, c, ROUND);
-        sum += exp2_parts(fma(z, c, ROUND - n), n);
-        flags |= (!in && x[j] >= from ? 1u : 0u) << j;
-      }
-      sum = wave_sum(sum);
-      if (lane == 0) sh.seg_mass[i] = sum;
-      return flags;
-    });
-    selected = n_list <= LIST;
-    if (selected) {
-      double own = 0., sure_mass;
-      for (int i = act_begin; i < act_end; ++i) own += sh.seg_mass[i];
-      sh.row.scan.exclusive(own, sure_mass);
-      if (use_k && bin_high >= 0) select_count(want, n_list);
-      if (use_p) select_mass(s.top_p * row.all_mass - sure_mass);
-      end_of_ties();
-      for (int i = act_begin; i < act_end; ++i) {
-        double w = sh.seg_mass[i];
-        const int stop = i + 1 < n_active ? sh.seg_first[i + 1] : n_list;
-        for (int j = sh.seg_first[i]; j < stop; ++j) w += entry_weight(j);
-        sh.seg_mass[i] = w;
-      }
+      if (lane == 0) sh.limits[wave] = limit;
     }
+    __syncthreads();
+    sure = sh.limits[0];
+    from = sh.limits[1];
+    want = use_k ? s.top_k - (int64_t)sh.above : 0;
   }
-  if (!selected) {
+  // Mass of a segment's logits from `sure` on; flags: those for the list.
+  DEVI double sure_mass(const float (&x)[SEG_LANE], float sure, float from, unsigned& flags) const {
+    const float nowhere = (float)fmax(m - 1000. / s.c, -3.402823466e38);  // 2^-1000 of the maximum, or next to it
+    double sum = 0.;
+    flags = 0;
+#pragma unroll
+    for (int j = 0; j < SEG_LANE; ++j) {
+      const bool in = x[j] >= sure;
+      const double z = (double)stat_max(in ? x[j] : nowhere, nowhere) - m, n = fma(z, s.c, ROUND);
+      sum += exp2_parts(fma(z, s.c, ROUND - n), n);
+      flags |= (!in && x[j] >= from ? 1u : 0u) << j;
+    }
+    return wave_sum(sum);
+  }
+  // With the masses in seg_mass and the list complete.
+  DEVI void many(int64_t want) {
+    if (want != NO_INDEX) {
+      double own = 0., sure;
+      for (int i = begin_active; i < end_active; ++i) own += sh.seg_mass[i];
+      sh.row.scan.exclusive(own, sure);
+      if (use_k) select_count(want);
+      else select_mass(s.top_p * all_mass - sure);
+      weigh_list();
+      for (int i = begin_active; i < end_active; ++i) sh.seg_mass[i] += list_mass(i);
+    }
+    pick_from_segments();
+  }
+  // Anything else: radix selection over the segments.
+  DEVI void any() {
     listed = false;
     if (use_k) {
       int own = 0, all;
       each([&](uint32_t) { ++own; });
       sh.ints.exclusive(own, all);
-      if (all > s.top_k) select_count(s.top_k, all);
+      if (all > s.top_k) select_count(s.top_k);
     }
-    if (use_p) select_mass(s.top_p * row.all_mass);
+    if (use_p) select_mass(s.top_p * all_mass);
     apply_min_p();
     sweep([&](const float (&x)[SEG_LANE], int i) {
       int n = 0;
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j) n += x[j] >= low && key_of(x[j]) == cut_key;
       n = wave_sum(n);
-      if (lane == 0) sh.seg_first[i] = n;
+      if (lane == 0) sh.seg_count[i] = n;
     });
-    if (tid == 0) sh.bin = -1;
     __syncthreads();
-    int n = 0, total;
-    for (int i = act_begin; i < act_end; ++i) n += sh.seg_first[i];
-    int cum = sh.ints.exclusive(n, total);
-    for (int i = act_begin; i < act_end; ++i) {
-      if (cum < take && take <= cum + sh.seg_first[i]) {
-        sh.bin = i;
-        sh.ties = take - cum;
-      }
-      cum += sh.seg_first[i];
-    }
-    __syncthreads();
-    if (wave == 0 && sh.bin >= 0) {  // the segment in which the last tie lies
+    find_last_tie([&](int i) { return sh.seg_count[i]; });
+    if (wave == 0 && sh.bin >= 0) {
       const int i = sh.bin;
       float x[SEG_LANE];
       Raw<E> raw;
@@ -1008,12 +1062,11 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       order_in_wave<E>(flags, starts);
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j)
-        if ((flags >> j & 1) && order_of<E>(flags, starts, j) + 1 == sh.ties)
-          sh.cut_index = (int)sh.active[i] * SEG + place_of<E>(j, lane);
+        if ((flags >> j & 1) && order_of<E>(flags, starts, j) + 1 == sh.ties) sh.cut_index = base_of(i) + place_of<E>(j, lane);
     }
     __syncthreads();
     sweep([&](const float (&x)[SEG_LANE], int i) {
-      const int base = (int)sh.active[i] * SEG;
+      const int base = base_of(i);
       double sum = 0.;
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j)
@@ -1021,26 +1074,211 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
       sum = wave_sum(sum);
       if (lane == 0) sh.seg_mass[i] = sum;
     });
+    __syncthreads();
+    pick_from_segments();
+  }
+  DEVI void pick_from_segments() {
+    double own = 0., z;
+    for (int i = begin_active; i < end_active; ++i) own += sh.seg_mass[i];
+    const double front = sh.row.scan.exclusive(own, z), target = u * z;
+    const int chosen = Base::choose(begin_active, end_active, front, target, [&](int i) { return sh.seg_mass[i]; });
+    if (wave == 0) {
+      const int base = base_of(chosen);
+      float x[SEG_LANE];
+      double w[SEG_LANE];
+      Raw<E> raw;
+      load_active(chosen, raw);
+      widen_raw<E>(raw, x);
+#pragma unroll
+      for (int j = 0; j < SEG_LANE; ++j)
+        w[j] = x[j] >= low ? kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane)) : 0.;
+      const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
+      if (lane == 0) finish_cut(token, z);
+    }
+  }
+};
+
+// A workgroup per row. SPREAD: rows with many candidates are left to the two kernels below.
+template <class E, int THREADS, int SEGS, bool SPREAD>
+__global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t row0) {
+  __shared__ CutShared<THREADS, SEGS> sh;
+  Cut<E, THREADS, SEGS> cut(a, sh, row0, blockIdx.x);
+  if (SPREAD && threadIdx.x == 0) a.spread[blockIdx.x].state = 0;
+  if (!cut.combine() || cut.simple()) return;
+  cut.bound();
+  cut.collect([&](const float (&x)[SEG_LANE], int) {
+    unsigned flags = 0;
+#pragma unroll
+    for (int j = 0; j < SEG_LANE; ++j) flags |= (x[j] >= cut.low ? 1u : 0u) << j;
+    return flags;
+  });
+  if (cut.n_list <= LIST) return cut.few();
+  if (!cut.can_bin()) return cut.any();
+  if (SPREAD) {
+    if (threadIdx.x == 0) {
+      Spread& s = a.spread[blockIdx.x];
+      s.low = cut.low;
+      s.top = cut.top;
+      s.all_mass = cut.all_mass;
+      s.state = 1;
+    }
+    return;
+  }
+  float sure = cut.low, from = pos_inf();
+  int64_t want = NO_INDEX;
+  if (cut.use_k || cut.use_p) {
+    cut.prepare_bins();
+    cut.fill_bins();
+    unsigned long long h[cut.OWN];
+#pragma unroll
+    for (int i = 0; i < cut.OWN; ++i) h[i] = sh.bins[threadIdx.x * cut.OWN + i];
+    cut.bracket(h, sure, from, want);
   }
   __syncthreads();
-  double own = 0., z;
-  for (int i = act_begin; i < act_end; ++i) own += sh.seg_mass[i];
-  const double front = sh.row.scan.exclusive(own, z);
-  const double target = row.u * z;
-  const int chosen = row.choose(act_begin, act_end, front, target, [&](int i) { return sh.seg_mass[i]; });
-  if (wave == 0) {
-    const int base = (int)sh.active[chosen] * SEG;
-    float x[SEG_LANE];
-    double w[SEG_LANE];
-    Raw<E> raw;
-    load_active(chosen, raw);
-    widen_raw<E>(raw, x);
-#pragma unroll
-    for (int j = 0; j < SEG_LANE; ++j)
-      w[j] = x[j] >= low ? kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane)) : 0.;
-    const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
-    if (lane == 0) row.finish(token, z, cut_key == 0 ? low : value_of(cut_key), sh.cut_index);
+  if (threadIdx.x == 0) sh.n_list = 0;
+  __syncthreads();
+  cut.collect([&](const float (&x)[SEG_LANE], int i) {
+    unsigned flags;
+    const double sum = cut.sure_mass(x, sure, from, flags);
+    if (cut.lane == 0) sh.seg_mass[i] = sum;
+    return flags;
+  });
+  if (cut.n_list <= LIST) cut.many(want);
+  else cut.any();
+}
+
+// What a workgroup of a spread row starts with. False: the row is not spread.
+template <class E, int THREADS, int SEGS>
+DEVI bool resume(Cut<E, THREADS, SEGS>& cut, const Spread& s) {
+  if (s.state != 1) return false;
+  cut.top = s.top;
+  cut.m = s.top;
+  cut.low = s.low;
+  cut.all_mass = s.all_mass;
+  cut.u = cut.uniform();
+  cut.top_key = key_of(cut.top);
+  cut.range_of_keys();
+  if (threadIdx.x == 0) {
+    cut.sh.row.first = NO_INDEX;
+    cut.sh.row.last = -1;
   }
+  return true;
+}
+// The segments [part * PART, ...) that reach the lower bound, as the active ones.
+template <class E, int THREADS, int SEGS>
+DEVI void activate_part(Cut<E, THREADS, SEGS>& cut, int part) {
+  const int begin = part * PART, n = min(PART, cut.a.segs - begin);
+  if (cut.wave == 0) {
+    const bool in = cut.lane < n && cut.seg_max[begin + cut.lane] >= cut.low;
+    const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
+    if (in) cut.sh.active[__popcll(all & ((1ull << cut.lane) - 1))] = (unsigned short)(begin + cut.lane);
+    if (cut.lane == 0) cut.sh.ties = __popcll(all);
+  }
+  __syncthreads();
+  cut.n_active = cut.sh.ties;
+  cut.share_active();
+}
+
+// Spread rows take four launches (what workgroups on several XCDs hand to each other inside one launch needs their L2s
+// written back: 640 of them took 93 us for this kernel). First a workgroup bins PART segments.
+template <class E>
+__global__ __launch_bounds__(1024) void sample_bins_kernel(Call a, int64_t row0, int parts) {
+  __shared__ CutShared<1024, FEW_SEGS> sh;
+  const unsigned r = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - r * (unsigned)parts);
+  Cut<E, 1024, FEW_SEGS> cut(a, sh, row0, r);
+  if (!resume(cut, a.spread[r]) || (!cut.use_k && !cut.use_p)) return;
+  cut.prepare_bins();
+  activate_part(cut, part);
+  cut.fill_bins();
+  unsigned long long* const bins = a.part_bins + ((int64_t)r * parts + part) * BINS;
+  for (int i = threadIdx.x; i < BINS; i += 1024) bins[i] = sh.bins[i];
+}
+// Second, a workgroup per row: the limits.
+template <class E>
+__global__ __launch_bounds__(1024) void sample_limits_kernel(Call a, int64_t row0, int parts) {
+  __shared__ CutShared<1024, FEW_SEGS> sh;
+  const unsigned r = blockIdx.x;
+  Spread& spread = a.spread[r];
+  Cut<E, 1024, FEW_SEGS> cut(a, sh, row0, r);
+  if (!resume(cut, spread)) return;
+  float sure = cut.low, from = pos_inf();
+  int64_t want = NO_INDEX;
+  if (cut.use_k || cut.use_p) {
+    cut.prepare_bins();
+    unsigned long long h[cut.OWN];
+#pragma unroll
+    for (int i = 0; i < cut.OWN; ++i) h[i] = 0;
+    const unsigned long long* const bins = a.part_bins + (int64_t)r * parts * BINS + threadIdx.x * cut.OWN;
+    for (int p = 0; p < parts; ++p) {
+#pragma unroll
+      for (int i = 0; i < cut.OWN; ++i) h[i] += bins[(int64_t)p * BINS + i];
+    }
+    cut.bracket(h, sure, from, want);
+  }
+  if (threadIdx.x == 0) {
+    spread.sure = sure;
+    spread.from = from;
+    spread.want = want;
+    spread.n_list = 0;
+  }
+}
+// Third, a workgroup adds up PART segments and lists the logits that the cut decides on.
+template <class E>
+__global__ __launch_bounds__(1024) void sample_masses_kernel(Call a, int64_t row0, int parts) {
+  __shared__ CutShared<1024, FEW_SEGS> sh;
+  constexpr int G = SEG_LANE / E::VEC;
+  const unsigned r = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - r * (unsigned)parts);
+  Spread& spread = a.spread[r];
+  Cut<E, 1024, FEW_SEGS> cut(a, sh, row0, r);
+  if (!resume(cut, spread)) return;
+  const float sure = spread.sure, from = spread.from;
+  activate_part(cut, part);
+  cut.sweep([&](const float (&x)[SEG_LANE], int i) {
+    unsigned flags;
+    const double sum = cut.sure_mass(x, sure, from, flags);
+    int starts[G];
+    const int own = order_in_wave<E>(flags, starts);
+    int to = 0;
+    if (cut.lane == 0) {
+      if (own > 0) to = atomicAdd(&spread.n_list, own);
+      const int64_t at = (int64_t)r * a.segs + sh.active[i];
+      a.part_mass[at] = sum;
+      a.part_runs[at] = make_int2(to, own);
+    }
+    to = __builtin_amdgcn_readfirstlane(to);
+    if (flags != 0) cut.append(x, flags, starts, to, cut.base_of(i), a.part_list + (int64_t)r * LIST, nullptr);
+  });
+}
+// Fourth, a workgroup per row: the cut and the token.
+template <class E>
+__global__ __launch_bounds__(1024) void sample_finish_kernel(Call a, int64_t row0) {
+  __shared__ CutShared<1024, FEW_SEGS> sh;
+  const unsigned r = blockIdx.x;
+  const Spread& spread = a.spread[r];
+  Cut<E, 1024, FEW_SEGS> cut(a, sh, row0, r);
+  if (!resume(cut, spread)) return;
+  const int seg = threadIdx.x;  // (FEW_SEGS are fewer than threads)
+  const bool in = seg < a.segs && cut.seg_max[seg] >= cut.low;
+  const int at = sh.ints.exclusive(in, cut.n_active);
+  if (in) {
+    const int2 run = a.part_runs[(int64_t)r * a.segs + seg];
+    sh.active[at] = (unsigned short)seg;
+    sh.seg_mass[at] = a.part_mass[(int64_t)r * a.segs + seg];
+    sh.seg_first[at] = run.x;
+    sh.seg_count[at] = run.y;
+  }
+  cut.share_active();
+  cut.n_list = spread.n_list;
+  if (cut.n_list > LIST) return cut.any();
+  for (int i = threadIdx.x; i < cut.n_list; i += 1024) {
+    const uint2 e = a.part_list[(int64_t)r * LIST + i];
+    sh.entry[i].x = e.x;
+    sh.index[i] = (int)e.y;
+  }
+  __syncthreads();
+  cut.many(spread.want);
 }
 
 // The kept sets as bits, a wave per segment (32 words); segments below the cut are not read.
@@ -1081,7 +1319,7 @@ int64_t rows_per_launch(int64_t rows, int64_t segs) {
   return std::min(rows, std::max<int64_t>((int64_t)(1 << 22) / segs, 1));
 }
 struct Layout {
-  int64_t rows, seg_max, seg_sum, sub_max, cut, cut_index, bytes;
+  int64_t rows, seg_max, seg_sum, sub_max, cut, cut_index, parts, spread, part_bins, part_mass, part_runs, part_list, bytes;
   Layout(int64_t n, int64_t V) {
     const int64_t segs = ceil_div_i64(V, SEG);
     rows = rows_per_launch(n, segs);
@@ -1096,6 +1334,12 @@ struct Layout {
     sub_max = take(rows * segs * SUBS * 4);
     cut = take(rows * 4);
     cut_index = take(rows * 4);
+    parts = segs <= FEW_SEGS && n <= SPREAD_ROWS ? ceil_div_i64(segs, PART) : 0;
+    spread = take(parts ? rows * (int64_t)sizeof(Spread) : 0);
+    part_bins = take(rows * parts * BINS * 8);
+    part_mass = take(parts ? rows * segs * 8 : 0);
+    part_runs = take(parts ? rows * segs * 8 : 0);
+    part_list = take(parts ? rows * LIST * 8 : 0);
     bytes = at;
   }
 };
@@ -1106,6 +1350,8 @@ int launch_sample(Call a, int64_t n, const Layout& l, hipStream_t stream) {
   const bool whole = (a.temperature_rows == nullptr && a.temperature <= 0.) ||
                      (a.top_k_rows == nullptr && a.top_p_rows == nullptr && a.min_p_rows == nullptr &&
                       (a.top_k == 1 || a.top_p <= 0. || ((a.top_k <= 0 || a.top_k >= a.V) && a.top_p >= 1. && a.min_p <= 0.)));
+  // few rows, unless top-k keeps every row's candidates few
+  const bool spread = l.parts > 0 && (a.top_k_rows != nullptr || a.top_k <= 0 || a.top_k > (int64_t)a.segs * SUBS);
   for (int64_t row0 = 0; row0 < n; row0 += l.rows) {
     const int64_t rows = std::min(l.rows, n - row0);
     const unsigned units = (unsigned)(rows * a.segs), blocks = (units + 3) / 4;
@@ -1119,14 +1365,29 @@ int launch_sample(Call a, int64_t n, const Layout& l, hipStream_t stream) {
       segments(std::integral_constant<int, 4>{});
     else
       segments(std::integral_constant<int, 1>{});
-    if (whole)
+    auto row_kernel = [&](auto threads, auto segs, auto spread) {
+      constexpr int THREADS = decltype(threads)::value;
+      hipLaunchKernelGGL((sample_rows_kernel<E, THREADS, decltype(segs)::value, decltype(spread)::value>),
+                         dim3((unsigned)rows), dim3(THREADS), 0, stream, a, row0);
+    };
+    const std::integral_constant<int, 1024> wide;
+    const std::integral_constant<int, FEW_SEGS> few;
+    if (whole) {
       hipLaunchKernelGGL((sample_whole_kernel<E>), dim3((unsigned)rows), dim3(256), 0, stream, a, row0);
-    else if (a.segs > FEW_SEGS)
-      hipLaunchKernelGGL((sample_rows_kernel<E, 1024, MAX_SEGS>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
-    else if (rows > FEW_ROWS)
-      hipLaunchKernelGGL((sample_rows_kernel<E, 512, FEW_SEGS>), dim3((unsigned)rows), dim3(512), 0, stream, a, row0);
-    else
-      hipLaunchKernelGGL((sample_rows_kernel<E, 1024, FEW_SEGS>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
+    } else if (spread) {
+      const unsigned parts = (unsigned)(rows * l.parts);
+      row_kernel(wide, few, std::true_type{});
+      hipLaunchKernelGGL((sample_bins_kernel<E>), dim3(parts), dim3(1024), 0, stream, a, row0, (int)l.parts);
+      hipLaunchKernelGGL((sample_limits_kernel<E>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0, (int)l.parts);
+      hipLaunchKernelGGL((sample_masses_kernel<E>), dim3(parts), dim3(1024), 0, stream, a, row0, (int)l.parts);
+      hipLaunchKernelGGL((sample_finish_kernel<E>), dim3((unsigned)rows), dim3(1024), 0, stream, a, row0);
+    } else if (a.segs > FEW_SEGS) {
+      row_kernel(wide, std::integral_constant<int, MAX_SEGS>{}, std::false_type{});
+    } else if (rows > FEW_ROWS) {
+      row_kernel(std::integral_constant<int, 512>{}, few, std::false_type{});
+    } else {
+      row_kernel(wide, few, std::false_type{});
+    }
     if (a.kept != nullptr)
       hipLaunchKernelGGL((sample_kept_kernel<E>), dim3(blocks), dim3(256), 0, stream, a, units, row0);
     AREAL_CHECK_LAUNCH();
@@ -1171,6 +1432,13 @@ int areal_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t N, in
   while ((1ll << (62 - a.fixed_bits - 1)) >= V && a.fixed_bits < 51) ++a.fixed_bits;  // V weights of at most 1 stay below 2^62
   a.tokens = tokens; a.logprobs = logprobs; a.full_logprobs = full_logprobs; a.kept = kept; a.kept_ld = kept_ld;
   a.seg_sum = (double*)(ws + l.seg_sum); a.seg_max = (float*)(ws + l.seg_max); a.sub_max = (float*)(ws + l.sub_max);
+  if (l.parts > 0) {
+    a.spread = (Spread*)(ws + l.spread);
+    a.part_bins = (unsigned long long*)(ws + l.part_bins);
+    a.part_mass = (double*)(ws + l.part_mass);
+    a.part_runs = (int2*)(ws + l.part_runs);
+    a.part_list = (uint2*)(ws + l.part_list);
+  }
   a.cut = (float*)(ws + l.cut); a.cut_index = (int*)(ws + l.cut_index);
   if (dtype == 0) return launch_sample<F32>(a, N, l, stream);
   if (dtype == 1) return launch_sample<BF16>(a, N, l, stream);
