@@ -336,24 +336,22 @@ DEVI int wave_pick(const double (&w)[SEG_LANE], int seg_base, double base, doubl
 }
 
 // Positions of flagged elements (bit i of `flags`: element i of the lane) in index order: starts[g] of a lane's first in
-// group g. Returns the wave's number of them.
+// group g. Returns the wave's number of them. Two groups' counts, of at most 512, go through one scan.
 template <class E>
 DEVI int order_in_wave(unsigned flags, int (&starts)[SEG_LANE / E::VEC]) {
   constexpr int VEC = E::VEC, G = SEG_LANE / VEC;
   int at = 0;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int n = __popc((flags >> (g * VEC)) & ((1u << VEC) - 1));
-    const int incl = wave_inclusive_scan(n, 0, [](int x, int y) { return x + y; });
-    starts[g] = at + incl - n;
-    at += lane_value(incl, 63);
+  for (int g = 0; g < G; g += 2) {
+    const int n0 = __popc((flags >> (g * VEC)) & ((1u << VEC) - 1)), n1 = __popc((flags >> ((g + 1) * VEC)) & ((1u << VEC) - 1));
+    const int incl = wave_inclusive_scan(n0 | n1 << 16, 0, [](int x, int y) { return x + y; });
+    const int all = lane_value(incl, 63);
+    starts[g] = at + (incl & 0xffff) - n0;
+    at += all & 0xffff;
+    starts[g + 1] = at + (incl >> 16) - n1;
+    at += all >> 16;
   }
   return at;
-}
-template <class E>
-DEVI int order_of(unsigned flags, const int (&starts)[SEG_LANE / E::VEC], int i) {
-  constexpr int VEC = E::VEC;
-  return starts[i / VEC] + __popc((flags >> (i / VEC * VEC)) & ((1u << (i % VEC)) - 1));
 }
 
 // ---- second pass, a workgroup per row ----
@@ -366,9 +364,10 @@ struct RowShared {
 };
 constexpr int NO_INDEX = 0x7fffffff;
 
-// A row's segments in the hands of THREADS threads, `per` consecutive ones each.
-template <class E, int THREADS>
+// A row's segments in the hands of THREADS threads, `per` consecutive ones each (up to PER, kept in registers).
+template <class E, int THREADS, int SEGS>
 struct Row {
+  static constexpr int PER = (SEGS + THREADS - 1) / THREADS;
   static constexpr int WAVES = THREADS / 64;
   const Call& a;
   RowShared<THREADS>& sh;
@@ -380,6 +379,8 @@ struct Row {
   const double* const seg_sum;
   const Settings s;
   int begin, end;
+  float own_max[PER];
+  double own_mass[PER];
   float top;
   double m, u, all_mass, before;
 
@@ -387,8 +388,6 @@ struct Row {
       : a(call), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63), wave(threadIdx.x >> 6), r(row_in_launch),
         row(row0 + row_in_launch), x_row((const typename E::S*)a.logits + row * a.ld),
         seg_max(a.seg_max + (int64_t)r * a.segs), seg_sum(a.seg_sum + (int64_t)r * a.segs), s(settings_of(a, row)) {}
-
-  DEVI double seg_mass(int i) const { return seg_sum[i] * weight_of(seg_max[i], m, s.c); }
 
   DEVI double uniform() const {
     const double v = a.wide_uniforms ? ((const double*)a.uniforms)[row] : (double)((const float*)a.uniforms)[row];
@@ -401,7 +400,14 @@ struct Row {
     begin = min(tid * per, a.segs);
     end = min(begin + per, a.segs);
     top = neg_inf();
-    for (int i = begin; i < end; ++i) top = stat_max(top, seg_max[i]);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = begin + i < end;
+      own_max[i] = in ? seg_max[begin + i] : neg_inf();
+      own_mass[i] = in ? seg_sum[begin + i] : 0.;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) top = stat_max(top, own_max[i]);
     top = wave_stat_max(top);
     if (tid == 0) {
       sh.first = NO_INDEX;
@@ -426,44 +432,55 @@ struct Row {
     }
     m = top;
     double own = 0.;
-    for (int i = begin; i < end; ++i) own += seg_mass(i);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      own_mass[i] *= weight_of(own_max[i], m, s.c);
+      own += own_mass[i];
+    }
     before = sh.scan.exclusive(own, all_mass);
     return true;
   }
 
-  // Results, by one thread. z: the mass of the kept set.
+  // Results, by one wave (with the same arguments in lanes 0 and 1). z: the mass of the kept set.
   DEVI void finish(int token, double z, float cut, int cut_index) const {
+    if (lane > 1) return;
     constexpr double LN2 = 0.6931471805599453;
     const double d = ((double)E::one(x_row[token]) - m) * s.c;
-    a.tokens[row] = token;
-    a.logprobs[row] = (float)(s.top1 ? 0. : fma(d, LN2, -log(z)));
-    a.full_logprobs[row] = (float)(s.greedy ? 0. : fma(d, LN2, -log(all_mass)));
-    a.cut[r] = cut;
-    a.cut_index[r] = cut_index;
+    const double lp = fma(d, LN2, -log(lane == 0 ? z : all_mass));
+    if (lane == 0) {
+      a.logprobs[row] = (float)(s.top1 ? 0. : lp);
+      a.tokens[row] = token;
+      a.cut[r] = cut;
+      a.cut_index[r] = cut_index;
+    } else {
+      a.full_logprobs[row] = (float)(s.greedy ? 0. : lp);
+    }
   }
 
-  // Which of n consecutive masses the target lies in, a run [i0, i1) of them with a thread; sh.target = their sum in front
-  // of it. All threads get it.
-  template <class F>
-  DEVI int choose(int i0, int i1, double front, double target, F mass) {
+  // Which of n consecutive masses the target lies in, i0, ... (up to PER, 0 behind the last) with a thread; sh.target =
+  // their sum in front of it. All threads get it.
+  DEVI int choose(int i0, const double (&mass)[PER], double front, double target) {
     double cum = front;
-    for (int i = i0; i < i1; ++i) {
-      const double w = mass(i);
-      if (w > 1e-200) {  // (a segment without a kept logit may have a mass of 1024 times 2^-1000)
-        if (cum + w > target) {
-          atomicMin(&sh.first, i);
-          break;
+    bool open = true;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (open && mass[i] > 1e-200) {  // (a segment without a kept logit may have a mass of 1024 times 2^-1000)
+        if (cum + mass[i] > target) {
+          atomicMin(&sh.first, i0 + i);
+          open = false;
+        } else {
+          atomicMax(&sh.last, i0 + i);
         }
-        atomicMax(&sh.last, i);
       }
-      cum += w;
+      cum += mass[i];
     }
     __syncthreads();
     const int at = sh.first != NO_INDEX ? sh.first : sh.last;
-    if (at >= i0 && at < i1) {
-      cum = front;
-      for (int i = i0; i < at; ++i) cum += mass(i);
-      sh.target = cum;
+    cum = front;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (i0 + i == at && mass[i] > 0.) sh.target = cum;
+      cum += mass[i];
     }
     __syncthreads();
     return at;
@@ -472,11 +489,9 @@ struct Row {
   // The settings that need no selection. False: others.
   DEVI bool simple() {
     if (s.top1) {  // the lowest index of the largest logit
-      for (int i = begin; i < end; ++i)
-        if (seg_max[i] == top) {
-          atomicMin(&sh.first, i);
-          break;
-        }
+#pragma unroll
+      for (int i = PER - 1; i >= 0; --i)
+        if (own_max[i] == top) atomicMin(&sh.first, begin + i);
       __syncthreads();
       if (wave == 0) {
         const int seg = sh.first;
@@ -487,14 +502,14 @@ struct Row {
         for (int i = SEG_LANE - 1; i >= 0; --i)
           if (x[i] == top) at = seg * SEG + place_of<E>(i, lane);
         at = wave_reduce(at, [](int p, int q) { return p < q ? p : q; });
-        if (lane == 0) finish(at, 1., top, at);
+        finish(at, 1., top, at);
       }
       return true;
     }
     if (s.top_k < a.V || s.top_p < 1. || s.min_p > 0.) return false;
     // the whole distribution: only the segment with the target is read again
     const double target = u * all_mass;
-    const int seg = choose(begin, end, before, target, [&](int i) { return seg_mass(i); });
+    const int seg = choose(begin, own_mass, before, target);
     if (wave == 0) {
       float x[SEG_LANE];
       double w[SEG_LANE];
@@ -502,21 +517,22 @@ struct Row {
 #pragma unroll
       for (int i = 0; i < SEG_LANE; ++i) w[i] = weight_of(x[i], m, s.c);
       const int token = wave_pick<E>(w, seg * SEG, sh.target, target, lane);
-      if (lane == 0) finish(token, all_mass, neg_inf(), -1);
+      finish(token, all_mass, neg_inf(), -1);
     }
     return true;
   }
 };
 
 // Calls without a limit in any row.
-template <class E>
+template <class E, int SEGS>
 __global__ __launch_bounds__(256) void sample_whole_kernel(Call a, int64_t row0) {
   __shared__ RowShared<256> sh;
-  Row<E, 256> row(a, sh, row0, blockIdx.x);
+  Row<E, 256, SEGS> row(a, sh, row0, blockIdx.x);
   if (row.combine()) row.simple();
 }
 
 constexpr int BINS = 2048;
+constexpr unsigned STEPS = 1024;
 constexpr int PART = 16;  // segments of a workgroup where a row is spread over several: one per wave
 
 template <int THREADS, int SEGS>
@@ -525,18 +541,19 @@ struct CutShared {
   RowShared<THREADS> row;
   BlockScan<WAVES, int> ints;
   BlockScan<WAVES, unsigned long long> wide;
-  union {
-    unsigned long long mass[256];
-    uint32_t count[256];
-  };
   unsigned long long above;
   int bin, ties, bin_low, bin_high, cut_index, n_list;
   float limits[2];
   unsigned short active[SEGS];  // segments that reach the lower bound
   int seg_first[SEGS], seg_count[SEGS];  // their entries of the list: a run of it each, in index order
+  int seg_ties[SEGS];
+  double seg_mass[SEGS];
   union {
     unsigned long long bins[BINS];
-    double seg_mass[SEGS];
+    struct {  // one of 256 bins for each round of a selection
+      unsigned long long mass[4][256];
+      uint32_t count[4][256], step_count[STEPS];
+    };
   };
   uint2 entry[LIST];  // .x: key, later the entry's weight in its place
   int index[LIST];
@@ -545,9 +562,10 @@ struct CutShared {
 // A row whose kept set is a proper prefix of the order: the set ends at a key (`cut_key`) and at an index among that key's
 // ties. THREADS threads work on it, or the workgroups of several launches.
 template <class E, int THREADS, int SEGS>
-struct Cut : Row<E, THREADS> {
+struct Cut : Row<E, THREADS, SEGS> {
   static constexpr int VEC = E::VEC, G = SEG_LANE / VEC, WAVES = THREADS / 64, LOW = E::LOW;
-  using Base = Row<E, THREADS>;
+  using Base = Row<E, THREADS, SEGS>;
+  static constexpr int PER = Base::PER;
   using Base::a; using Base::tid; using Base::lane; using Base::wave; using Base::r; using Base::s; using Base::m;
   using Base::top; using Base::all_mass; using Base::x_row; using Base::seg_max; using Base::u;
   CutShared<THREADS, SEGS>& sh;
@@ -590,19 +608,18 @@ struct Cut : Row<E, THREADS> {
     return to;
   }
 
-  DEVI void clear_bins() {  // 256 of them
-    __syncthreads();
-    for (int i = tid; i < 256; i += THREADS) sh.mass[i] = 0;
-    __syncthreads();
+  // All bins; a barrier has to follow.
+  DEVI void clear_bins() {
+    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
   }
   // The bin, from the 256th downwards, in which the running count reaches `want`: sh.bin, the count in front and its own.
-  DEVI void find_count(int64_t want) {
+  DEVI void find_count(const uint32_t (&count)[256], int64_t want) {
     __syncthreads();
     if (wave == 0) {
       uint32_t n4[4];
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) n += (int)(n4[i] = sh.count[255 - 4 * lane - i]);
+      for (int i = 0; i < 4; ++i) n += (int)(n4[i] = count[255 - 4 * lane - i]);
       const int incl = wave_inclusive_scan(n, 0, [](int x, int y) { return x + y; });
       if (incl - n < want && incl >= want) {
         int cum = incl - n;
@@ -630,6 +647,7 @@ struct Cut : Row<E, THREADS> {
 
   // A lower bound on the kept logits, so that few are looked at; the segments that reach it, in index order.
   DEVI void bound() {
+    clear_bins();
     top_key = key_of(top);
     low = -3.402823466e38f;
     if (use_p && !use_k) {
@@ -648,31 +666,35 @@ struct Cut : Row<E, THREADS> {
     }
     if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
       // top_k maxima of disjoint parts of the row are that many logits: the top_k-th largest of the row is no lower than
-      // theirs. Its upper 16 bits are enough.
+      // theirs. Counted in steps of 2^17 keys (a 64th of a binade) below the largest logit, the last step for all
+      // that is further down; the lower end of the top_k-th's will do.
       const float* subs = a.sub_max + (int64_t)r * a.segs * SUBS;
       const int n = a.segs * SUBS;
-      uint32_t prefix = 0;
-      int64_t want = s.top_k;
+      __syncthreads();  // (the bins are clear)
+      for (int i = tid; i < n; i += THREADS) atomicAdd(&sh.step_count[min((top_key - key_of(subs[i])) >> 17, STEPS - 1u)], 1u);
+      __syncthreads();
+      constexpr int MINE = STEPS / THREADS;
+      int count[MINE], own = 0, total;
 #pragma unroll
-      for (int shift = 24; shift >= 16; shift -= 8) {
-        clear_bins();
-        for (int i = tid; i < n; i += THREADS) {
-          const uint32_t key = key_of(subs[i]);
-          if (shift == 24 || (key >> 24) == (prefix >> 24)) atomicAdd(&sh.count[(key >> shift) & 255], 1u);
-        }
-        find_count(want);
-        prefix |= (uint32_t)sh.bin << shift;
-        want -= (int64_t)sh.above;
+      for (int i = 0; i < MINE; ++i) own += count[i] = (int)sh.step_count[tid * MINE + i];
+      int cum = sh.ints.exclusive(own, total);
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        if (cum < s.top_k && cum + count[i] >= s.top_k) sh.bin = tid * MINE + i;
+        cum += count[i];
       }
-      const float lowest = value_of(prefix);
-      if (lowest > low) low = lowest;  // (not where it is a NaN's pattern, below that of -inf)
+      __syncthreads();
+      const uint32_t down = (uint32_t)(sh.bin + 1) << 17;
+      if (sh.bin < (int)STEPS - 1 && top_key >= down) low = fmaxf(low, value_of(top_key - down + 1));  // (not a NaN's)
     }
     range_of_keys();
     int mine = 0;
-    for (int i = Base::begin; i < Base::end; ++i) mine += seg_max[i] >= low;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += Base::own_max[i] >= low;
     int at = sh.ints.exclusive(mine, n_active);
-    for (int i = Base::begin; i < Base::end; ++i)
-      if (seg_max[i] >= low) sh.active[at++] = (unsigned short)i;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (Base::own_max[i] >= low) sh.active[at++] = (unsigned short)(Base::begin + i);
     share_active();
   }
   DEVI void share_active() {
@@ -688,30 +710,36 @@ struct Cut : Row<E, THREADS> {
 
   DEVI int base_of(int i) const { return (int)sh.active[i] * SEG; }
   DEVI void load_active(int i, Raw<E>& x) const { load_raw<E>(x_row, base_of(i), a.V, lane, x); }
-  // f(logits, i) of active segment i, a wave each; the next one's loads are under way meanwhile
+  // f(logits, i) of active segment i, a wave each; the loads of AHEAD segments (4 KB) are under way at a time
+  static constexpr int AHEAD = VEC / 2;
   template <class F>
   DEVI void sweep(F f) {
-    Raw<E> now, next;
-    if (wave < n_active) load_active(wave, now);
-    for (int i = wave; i < n_active; i += WAVES) {
-      if (i + WAVES < n_active) load_active(i + WAVES, next);
-      float x[SEG_LANE];
-      widen_raw<E>(now, x);
-      f(x, i);
-      now = next;
+    for (int i0 = wave; i0 < n_active; i0 += AHEAD * WAVES) {
+      Raw<E> raw[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * WAVES < n_active) load_active(i0 + k * WAVES, raw[k]);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * WAVES < n_active) {
+          float x[SEG_LANE];
+          widen_raw<E>(raw[k], x);
+          f(x, i0 + k * WAVES);
+        }
     }
   }
   // Appends the logits marked by `flags` (bit j: element j of the lane) to a list, in index order from entry `to` on.
-  DEVI void append(const float (&x)[SEG_LANE], unsigned flags, const int (&starts)[G], int to, int base, uint2* entry,
+  DEVI void append(const float (&x)[SEG_LANE], unsigned flags, int (&starts)[G], int to, int base, uint2* entry,
                    int* index) const {
 #pragma unroll
     for (int j = 0; j < SEG_LANE; ++j) {
-      const int p = to + order_of<E>(flags, starts, j);
-      if ((flags >> j & 1) && p < LIST) {
-        const int at = base + place_of<E>(j, lane);
-        entry[p].x = key_of(x[j]);
-        if (index != nullptr) index[p] = at;
-        else entry[p].y = (uint32_t)at;
+      if (flags >> j & 1) {
+        const int p = to + starts[j / VEC]++, at = base + place_of<E>(j, lane);
+        if (p < LIST) {
+          entry[p].x = key_of(x[j]);
+          if (index != nullptr) index[p] = at;
+          else entry[p].y = (uint32_t)at;
+        }
       }
     }
   }
@@ -756,19 +784,18 @@ struct Cut : Row<E, THREADS> {
     const double w = fma(weight_of(value_of(key), m, s.c), unit(), 4503599627370496.);
     return __builtin_bit_cast(unsigned long long, w) & 0xfffffffffffffull;
   }
-  // The key of the want-th largest candidate (of which there are more).
+  // The key of the want-th largest candidate (of which there are more); the bins are clear.
   DEVI void select_count(int64_t want) {
     uint32_t mask = common, prefix = top_key & common;
     int ties = 0;
-    int bits = top_bits;
+    int bits = top_bits, round = 0;
     do {
       const int shift = max(bits - 8, LOW);
       const uint32_t field = (1u << (max(bits, shift) - shift)) - 1;
-      clear_bins();
       each([&](uint32_t key) {
-        if ((key & mask) == prefix) atomicAdd(&sh.count[(key >> shift) & field], 1u);
+        if ((key & mask) == prefix) atomicAdd(&sh.count[round][(key >> shift) & field], 1u);
       });
-      find_count(want);
+      find_count(sh.count[round++], want);
       prefix |= (uint32_t)sh.bin << shift;
       mask = ~0u << shift;
       want -= (int64_t)sh.above;
@@ -779,24 +806,23 @@ struct Cut : Row<E, THREADS> {
     take = (int)want;
     tied_out = (unsigned long long)(ties - take) * fixed_mass(cut_key);
   }
-  // The key at which the candidates' mass reaches `least` (with top-k: top_p of S1's), within S1.
+  // The key at which the candidates' mass reaches `least` (with top-k: top_p of S1's), within S1; the bins are clear.
   DEVI void select_mass(double least) {
     uint32_t mask = common, prefix = top_key & common;
     unsigned long long want = 0;
-    int bits = top_bits;
+    int bits = top_bits, round = 0;
     bool first = true;
     do {
       const int shift = max(bits - 8, LOW);
       const uint32_t field = (1u << (max(bits, shift) - shift)) - 1;
-      clear_bins();
       each([&](uint32_t key) {
-        if ((key & mask) == prefix && key >= cut_key) atomicAdd(&sh.mass[(key >> shift) & field], fixed_mass(key));
+        if ((key & mask) == prefix && key >= cut_key) atomicAdd(&sh.mass[round][(key >> shift) & field], fixed_mass(key));
       });
       __syncthreads();
       if (wave == 0) {
         unsigned long long n4[4], n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += n4[i] = sh.mass[255 - 4 * lane - i];
+        for (int i = 0; i < 4; ++i) n += n4[i] = sh.mass[round][255 - 4 * lane - i];
         const unsigned long long incl =
             wave_inclusive_scan(n, 0ull, [](unsigned long long x, unsigned long long y) { return x + y; });
         if (first) {  // in S2: what has less than this in front of it
@@ -820,6 +846,7 @@ struct Cut : Row<E, THREADS> {
       }
       __syncthreads();
       first = false;
+      ++round;
       if (sh.bin < 0) return;  // less mass than that among the candidates: all of them stay
       prefix |= (uint32_t)sh.bin << shift;
       mask = ~0u << shift;
@@ -863,32 +890,52 @@ struct Cut : Row<E, THREADS> {
   DEVI double kept_weight(float x, uint32_t key, int at) const {
     return key > cut_key || (key == cut_key && at <= sh.cut_index) ? weight_of(x, m, s.c) : 0.;
   }
-  // The list's part of the kept set: weights in place of keys, added to the segments' masses.
+  // The list's part of the kept set: weights in place of keys, each segment's into its mass (ADD: added). Sixteen lanes
+  // per segment.
+  template <bool ADD>
   DEVI void weigh_list() {
-    auto ties = [&](int i) {
-      int n = 0;
-      for (int j = sh.seg_first[i]; j < sh.seg_first[i] + sh.seg_count[i]; ++j) n += sh.entry[j].x == cut_key;
-      return n;
-    };
     if (take != NO_INDEX) {
-      find_last_tie(ties);
-      if (sh.bin >= begin_active && sh.bin < end_active) {
-        int rank = 0, j = sh.seg_first[sh.bin];
-        while ((rank += sh.entry[j].x == cut_key) < sh.ties) ++j;
-        sh.cut_index = sh.index[j];
+      for (int i = tid / 16; i < n_active; i += THREADS / 16) {
+        int n = 0;
+        for (int j = tid % 16; j < sh.seg_count[i]; j += 16) n += sh.entry[sh.seg_first[i] + j].x == cut_key;
+        n = row_reduce(n, [](int x, int y) { return x + y; });
+        if (tid % 16 == 0) sh.seg_ties[i] = n;
+      }
+      __syncthreads();
+      find_last_tie([&](int i) { return sh.seg_ties[i]; });
+      if (wave == 0 && sh.bin >= 0) {
+        const int first = sh.seg_first[sh.bin], n = sh.seg_count[sh.bin];
+        int left = sh.ties;
+        for (int j = 0; j < n && left > 0; j += 64) {
+          const bool tie = j + lane < n && sh.entry[first + j + lane].x == cut_key;
+          const unsigned long long all = __builtin_amdgcn_ballot_w64(tie);
+          if (tie && __popcll(all & ((1ull << lane) - 1)) == left - 1) sh.cut_index = sh.index[first + j + lane];
+          left -= __popcll(all);
+        }
       }
       __syncthreads();
     }
-    for (int i = tid; i < n_list; i += THREADS) {
-      const uint32_t key = sh.entry[i].x;
-      sh.entry[i] = __builtin_bit_cast(uint2, kept_weight(value_of(key), key, sh.index[i]));
+    for (int i = tid / 16; i < n_active; i += THREADS / 16) {
+      double w = 0.;
+      for (int j = tid % 16; j < sh.seg_count[i]; j += 16) {
+        const int at = sh.seg_first[i] + j;
+        const uint32_t key = sh.entry[at].x;
+        const double e = kept_weight(value_of(key), key, sh.index[at]);
+        sh.entry[at] = __builtin_bit_cast(uint2, e);
+        w += e;
+      }
+      w = row_reduce(w, [](double x, double y) { return x + y; });
+      if (tid % 16 == 0) sh.seg_mass[i] = ADD ? sh.seg_mass[i] + w : w;
     }
     __syncthreads();
   }
-  DEVI double list_mass(int i) const {
-    double w = 0.;
-    for (int j = sh.seg_first[i]; j < sh.seg_first[i] + sh.seg_count[i]; ++j) w += __builtin_bit_cast(double, sh.entry[j]);
-    return w;
+  DEVI void load_masses(double (&mass)[PER], double& sum) const {
+    sum = 0.;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      mass[i] = begin_active + i < end_active ? sh.seg_mass[begin_active + i] : 0.;
+      sum += mass[i];
+    }
   }
   DEVI void finish_cut(int token, double z) const {
     // without a selection all from `low` on are kept
@@ -900,27 +947,25 @@ struct Cut : Row<E, THREADS> {
     if (use_k && n_list > s.top_k) select_count(s.top_k);
     if (use_p) select_mass(s.top_p * all_mass);
     apply_min_p();
-    weigh_list();
-    double own = 0., z;
-    for (int i = begin_active; i < end_active; ++i) {
-      const double w = list_mass(i);
-      sh.seg_mass[i] = w;
-      own += w;
-    }
+    weigh_list<false>();
+    double mass[PER], own, z;
+    load_masses(mass, own);
     const double front = sh.row.scan.exclusive(own, z), target = u * z;
-    const int chosen = Base::choose(begin_active, end_active, front, target, [&](int i) { return sh.seg_mass[i]; });
-    if (chosen >= begin_active && chosen < end_active) {
-      double cum = sh.row.target;
-      int token = -1;
-      for (int j = sh.seg_first[chosen]; j < sh.seg_first[chosen] + sh.seg_count[chosen]; ++j) {
-        const double w = __builtin_bit_cast(double, sh.entry[j]);
-        cum += w;
-        if (w > 0.) {
-          token = sh.index[j];
-          if (cum > target) break;
-        }
+    const int chosen = Base::choose(begin_active, mass, front, target);
+    if (wave == 0) {  // the entry in which the running mass passes the target, or the segment's last with a weight
+      const int first = sh.seg_first[chosen], n = sh.seg_count[chosen];
+      double base = sh.row.target;
+      int at = first;
+      for (int j = 0; j < n; j += 64) {
+        const double w = j + lane < n ? __builtin_bit_cast(double, sh.entry[first + j + lane]) : 0.;
+        const double incl = wave_inclusive_scan(w, 0., [](double x, double y) { return x + y; });
+        const unsigned long long some = __builtin_amdgcn_ballot_w64(w > 0.);
+        const unsigned long long cross = __builtin_amdgcn_ballot_w64(w > 0. && base + incl > target);
+        if (some != 0) at = first + j + (cross != 0 ? __builtin_ctzll(cross) : 63 - __builtin_clzll(some));
+        if (cross != 0) break;
+        base += lane_value(incl, 63);
       }
-      finish_cut(token, z);
+      finish_cut(sh.index[at], z);
     }
   }
 
@@ -941,7 +986,7 @@ struct Cut : Row<E, THREADS> {
   // Masses in 2^-32. A depth is off by 3 roundings of 2^-24 of at most 32 binades: 4e-6 of the exponential, whose own error
   // and truncation, 2^-23 and one unit, come to it.
   DEVI void fill_bins() {
-    for (int i = tid; i < BINS; i += THREADS) sh.bins[i] = 0;
+    clear_bins();
     __syncthreads();
     sweep([&](const float (&x)[SEG_LANE], int) {
 #pragma unroll
@@ -1019,19 +1064,20 @@ struct Cut : Row<E, THREADS> {
   // With the masses in seg_mass and the list complete.
   DEVI void many(int64_t want) {
     if (want != NO_INDEX) {
-      double own = 0., sure;
-      for (int i = begin_active; i < end_active; ++i) own += sh.seg_mass[i];
+      double mass[PER], own, sure;
+      load_masses(mass, own);
       sh.row.scan.exclusive(own, sure);
       if (use_k) select_count(want);
       else select_mass(s.top_p * all_mass - sure);
-      weigh_list();
-      for (int i = begin_active; i < end_active; ++i) sh.seg_mass[i] += list_mass(i);
+      weigh_list<true>();
     }
     pick_from_segments();
   }
   // Anything else: radix selection over the segments.
   DEVI void any() {
     listed = false;
+    clear_bins();
+    __syncthreads();
     if (use_k) {
       int own = 0, all;
       each([&](uint32_t) { ++own; });
@@ -1045,10 +1091,10 @@ struct Cut : Row<E, THREADS> {
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j) n += x[j] >= low && key_of(x[j]) == cut_key;
       n = wave_sum(n);
-      if (lane == 0) sh.seg_count[i] = n;
+      if (lane == 0) sh.seg_ties[i] = n;
     });
     __syncthreads();
-    find_last_tie([&](int i) { return sh.seg_count[i]; });
+    find_last_tie([&](int i) { return sh.seg_ties[i]; });
     if (wave == 0 && sh.bin >= 0) {
       const int i = sh.bin;
       float x[SEG_LANE];
@@ -1062,7 +1108,7 @@ struct Cut : Row<E, THREADS> {
       order_in_wave<E>(flags, starts);
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j)
-        if ((flags >> j & 1) && order_of<E>(flags, starts, j) + 1 == sh.ties) sh.cut_index = base_of(i) + place_of<E>(j, lane);
+        if ((flags >> j & 1) && ++starts[j / VEC] == sh.ties) sh.cut_index = base_of(i) + place_of<E>(j, lane);
     }
     __syncthreads();
     sweep([&](const float (&x)[SEG_LANE], int i) {
@@ -1078,10 +1124,10 @@ struct Cut : Row<E, THREADS> {
     pick_from_segments();
   }
   DEVI void pick_from_segments() {
-    double own = 0., z;
-    for (int i = begin_active; i < end_active; ++i) own += sh.seg_mass[i];
+    double mass[PER], own, z;
+    load_masses(mass, own);
     const double front = sh.row.scan.exclusive(own, z), target = u * z;
-    const int chosen = Base::choose(begin_active, end_active, front, target, [&](int i) { return sh.seg_mass[i]; });
+    const int chosen = Base::choose(begin_active, mass, front, target);
     if (wave == 0) {
       const int base = base_of(chosen);
       float x[SEG_LANE];
@@ -1093,7 +1139,7 @@ struct Cut : Row<E, THREADS> {
       for (int j = 0; j < SEG_LANE; ++j)
         w[j] = x[j] >= low ? kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane)) : 0.;
       const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
-      if (lane == 0) finish_cut(token, z);
+      finish_cut(token, z);
     }
   }
 };
@@ -1136,6 +1182,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(Call a, int64_t ro
   }
   __syncthreads();
   if (threadIdx.x == 0) sh.n_list = 0;
+  cut.clear_bins();
   __syncthreads();
   cut.collect([&](const float (&x)[SEG_LANE], int i) {
     unsigned flags;
@@ -1259,6 +1306,7 @@ __global__ __launch_bounds__(1024) void sample_finish_kernel(Call a, int64_t row
   const Spread& spread = a.spread[r];
   Cut<E, 1024, FEW_SEGS> cut(a, sh, row0, r);
   if (!resume(cut, spread)) return;
+  cut.clear_bins();
   const int seg = threadIdx.x;  // (FEW_SEGS are fewer than threads)
   const bool in = seg < a.segs && cut.seg_max[seg] >= cut.low;
   const int at = sh.ints.exclusive(in, cut.n_active);
@@ -1373,7 +1421,10 @@ int launch_sample(Call a, int64_t n, const Layout& l, hipStream_t stream) {
     const std::integral_constant<int, 1024> wide;
     const std::integral_constant<int, FEW_SEGS> few;
     if (whole) {
-      hipLaunchKernelGGL((sample_whole_kernel<E>), dim3((unsigned)rows), dim3(256), 0, stream, a, row0);
+      if (a.segs <= FEW_SEGS)
+        hipLaunchKernelGGL((sample_whole_kernel<E, FEW_SEGS>), dim3((unsigned)rows), dim3(256), 0, stream, a, row0);
+      else
+        hipLaunchKernelGGL((sample_whole_kernel<E, MAX_SEGS>), dim3((unsigned)rows), dim3(256), 0, stream, a, row0);
     } else if (spread) {
       const unsigned parts = (unsigned)(rows * l.parts);
       row_kernel(wide, few, std::true_type{});
