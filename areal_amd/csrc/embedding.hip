@@ -56,6 +56,10 @@ DEVI void store_pack(T* p, const Pack<T, VEC>& o) {
   }
 }
 
+// Loads that run ahead of their use have no condition: behind the row's or the list's end they repeat its first or last
+// piece. (Behind a branch each, the compiler waits for the one before: the 32 rows of embedding_sum_kernel one by one, 127
+// us for 32768 x 4096 bf16 that take 60.)
+
 // A wave takes ROW_PACKS packs per lane of one row: all loads before the first store.
 constexpr int ROW_PACKS = 4;
 template <typename W, typename O, int VEC>
@@ -75,7 +79,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const W* __restrict_
 #pragma unroll
   for (int i = 0; i < ROW_PACKS; ++i) {
     const int at = begin + i * 64 * VEC;
-    if (at < H) load_pack<W, VEC>(src + at, x[i]);
+    load_pack<W, VEC>(src + (at < H ? at : 0), x[i]);
   }
 #pragma unroll
   for (int i = 0; i < ROW_PACKS; ++i) {
@@ -91,6 +95,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const W* __restrict_
 
 // ---- the order of the tokens by id ----
 constexpr int SORT_WAVES = 16;
+constexpr int RANGE_BITS = 10;
 constexpr int RANGE_MAX = 768;  // ids of a workgroup: 16 waves' counts of them take 48 KB of LDS
 constexpr int SORT_UNROLL = 8;
 
@@ -109,29 +114,32 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const 
   for (int i = tid; i < SORT_WAVES * range; i += 64 * SORT_WAVES) counts[i] = 0;
   __syncthreads();
   int* const own = counts + wave * range;
-  const int run = (int)(((int64_t)T + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64)) * 64;
-  const int64_t t0 = (int64_t)wave * run, t1 = min(t0 + run, (int64_t)T);
-  // the place of an id in the range, -1 for others; SORT_UNROLL x 64 tokens at a time
+  // an odd number of 512-byte steps: with runs of 16 KB all waves of all workgroups read the same channel of an L2
+  const int run = (int)(((int64_t)T + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) | 1) * 64;
+  const int64_t t0 = min((int64_t)wave * run, (int64_t)T), t1 = min(t0 + run, (int64_t)T);
+  // f(token, id - lo as an unsigned number): below n for ids of the range, above -lo for lower ones; SORT_UNROLL x 64
+  // tokens at a time. (NONE, of ids that count nowhere, is neither: V is at most 2^31 - 2.)
+  constexpr uint32_t NONE = 0xffffffffu;
+  const uint32_t padding = padding_idx < 0 ? NONE : (uint32_t)padding_idx;
   auto sweep = [&](auto f) {
     for (int64_t t = t0; t < t1; t += SORT_UNROLL * 64) {
-      int64_t id[SORT_UNROLL];
+      uint2 raw[SORT_UNROLL];
 #pragma unroll
       for (int i = 0; i < SORT_UNROLL; ++i) {
         const int64_t at = t + i * 64 + lane;
-        id[i] = at < t1 ? ids[at] : -1;
+        raw[i] = at < t1 ? ((const uint2*)ids)[at] : make_uint2(NONE, NONE);
       }
 #pragma unroll
       for (int i = 0; i < SORT_UNROLL; ++i) {
-        const bool valid = id[i] >= 0 && id[i] < V && id[i] != padding_idx;
-        const int64_t rel = id[i] - lo;
-        f((int)(t + i * 64 + lane), valid && rel >= 0 && rel < n ? (int)rel : -1, valid && rel < 0);
+        const uint32_t id = raw[i].y == 0 && raw[i].x < (uint32_t)V && raw[i].x != padding ? raw[i].x : NONE;
+        f((int)(t + i * 64 + lane), id);
       }
     }
   };
   int below = 0;
-  sweep([&](int, int rel, bool lower) {
-    below += lower;
-    if (rel >= 0) atomicAdd(&own[rel], 1);
+  sweep([&](int, uint32_t id) {
+    below += id < (uint32_t)lo;
+    if (id - (uint32_t)lo < (uint32_t)n) atomicAdd(&own[id - (uint32_t)lo], 1);
   });
   below = wave_sum(below);
   if (lane == 0) below_of[wave] = below;
@@ -160,15 +168,23 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const 
   }
   __syncthreads();
   volatile int* const places = own;  // of this wave alone from here on
-  sweep([&](int t, int rel, bool) {
-    unsigned long long left = __builtin_amdgcn_ballot_w64(rel >= 0);
-    while (left != 0) {  // one id of the 64 tokens at a time
-      const int id = __builtin_amdgcn_readlane(rel, __builtin_ctzll(left));
-      const unsigned long long same = __builtin_amdgcn_ballot_w64(rel == id);
-      const int to = places[id];
-      if (rel == id) order[to + __popcll(same & ((1ull << lane) - 1))] = t;
-      if (lane == 0) places[id] = to + __popcll(same);
-      left &= ~same;
+  sweep([&](int t, uint32_t id) {
+    const uint32_t rel = id - (uint32_t)lo;
+    const bool in = rel < (uint32_t)n;
+    const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
+    if (all == 0) return;
+    // the lanes with this lane's id: those that agree with it in every bit (a hot range has a dozen ids among 64 tokens,
+    // one id at a time took 37 us of 85 at 32 Ki tokens)
+    unsigned long long same = all;
+#pragma unroll
+    for (int bit = 0; bit < RANGE_BITS; ++bit) {
+      const unsigned long long set = __builtin_amdgcn_ballot_w64(rel >> bit & 1);
+      same &= rel >> bit & 1 ? set : ~set;
+    }
+    if (in) {
+      const int to = places[rel], before = __popcll(same & ((1ull << lane) - 1));
+      order[to + before] = t;
+      if (before == 0) places[rel] = to + __popcll(same);
     }
   });
 }
@@ -183,6 +199,7 @@ struct Sums {
   const int *start, *order;
   float* partial;  // [runs][2][H]: of an id that began before the run; of one that began in it and goes on
   int T, V, H;
+  int* over;       // [runs]: the id that begins in the run and goes on behind it, or -1
   unsigned runs, slabs, sum_blocks;
   float scale;
 };
@@ -207,12 +224,13 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Sums a, const G* __r
     const int n = (int)min((int64_t)FILL_ROWS, a.V - v0);
     const bool empty = lane < n && a.start[v0 + lane] == a.start[v0 + lane + 1];
     unsigned long long left = __builtin_amdgcn_ballot_w64(empty);
-    Pack<D, VEC> zero;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) zero.v[j] = narrow1<D>(0.f);
     while (left != 0) {
       D* const row = dweight + (v0 + __builtin_ctzll(left)) * a.H;
-      for (int at = lane * VEC; at < a.H; at += 64 * VEC) store_pack<D, VEC>(row + at, zero);
+      constexpr int STEP = VEC == 1 ? 1 : 16 / sizeof(D);  // (whole lines of 16-byte stores, whatever the type)
+      for (int at = lane * STEP; at < a.H; at += 64 * STEP) {
+        if constexpr (VEC == 1) row[at] = narrow1<D>(0.f);
+        else *(u32x4*)(row + at) = u32x4{};
+      }
       left &= left - 1;
     }
     return;
@@ -225,6 +243,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Sums a, const G* __r
   const int n = min(RUN, valid - p0);
   const int column = (int)slab * 64 * VEC + lane * VEC;
   const bool inside = column < a.H;
+  const G* const grad_column = grad + (inside ? column : 0);
   // place i of the run: lane i
   int token = 0, id = -1, first = 0, end = 0;
   if (lane < n) {
@@ -233,6 +252,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Sums a, const G* __r
     first = a.start[id];
     end = a.start[id + 1];
   }
+  if (slab == 0 && lane == n - 1) a.over[run] = first >= p0 && end > p0 + RUN ? id : -1;
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
@@ -240,8 +260,8 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Sums a, const G* __r
     Pack<G, VEC> g[ROWS_AHEAD];
 #pragma unroll
     for (int i = 0; i < ROWS_AHEAD; ++i) {
-      const int t = __builtin_amdgcn_readlane(token, (i0 + i) & 63);
-      if (i0 + i < n && inside) load_pack<G, VEC>(grad + (int64_t)t * a.H + column, g[i]);
+      const int t = __builtin_amdgcn_readlane(token, min(i0 + i, n - 1));
+      load_pack<G, VEC>(grad_column + (int64_t)t * a.H, g[i]);
     }
 #pragma unroll
     for (int i = 0; i < ROWS_AHEAD; ++i) {
@@ -278,11 +298,9 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embedding_join_kernel(Sums a,
   __shared__ float sums[JOIN_WAVES][64 * VEC];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned run = blockIdx.x / a.slabs, slab = blockIdx.x - run * a.slabs;
-  const int next = ((int)run + 1) * RUN, valid = a.start[a.V];
-  if (next >= valid) return;
-  const int id = (int)a.ids[a.order[next - 1]];
-  const int first = a.start[id], end = a.start[id + 1];
-  if (end <= next || first < (int)run * RUN) return;
+  const int next = ((int)run + 1) * RUN, valid = a.start[a.V], id = a.over[run];
+  if (next >= valid || id < 0) return;  // (over is written up to the last run with a token)
+  const int end = a.start[id + 1];
   const int column = (int)slab * 64 * VEC + lane * VEC;
   const bool inside = column < a.H;
   // pieces: slot 1 of this run, then slot 0 of the `more` runs after it
@@ -292,21 +310,20 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void embedding_join_kernel(Sums a,
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  if (inside) {
-    for (int i0 = begin; i0 < stop; i0 += ROWS_AHEAD) {
-      Pack<float, VEC> g[ROWS_AHEAD];
+  const float* const partial = a.partial + (inside ? column : 0);
+  for (int i0 = begin; i0 < stop; i0 += ROWS_AHEAD) {
+    Pack<float, VEC> g[ROWS_AHEAD];
 #pragma unroll
-      for (int i = 0; i < ROWS_AHEAD; ++i) {
-        const int64_t slot = ((int64_t)run + i0 + i) * 2 + (i0 + i == 0 ? 1 : 0);
-        if (i0 + i < stop) load_pack<float, VEC>(a.partial + slot * a.H + column, g[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < ROWS_AHEAD; ++i)
-        if (i0 + i < stop) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] += g[i].v[j];
-        }
+    for (int i = 0; i < ROWS_AHEAD; ++i) {
+      const int piece = min(i0 + i, stop - 1);
+      load_pack<float, VEC>(partial + (((int64_t)run + piece) * 2 + (piece == 0 ? 1 : 0)) * a.H, g[i]);
     }
+#pragma unroll
+    for (int i = 0; i < ROWS_AHEAD; ++i)
+      if (i0 + i < stop) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += g[i].v[j];
+      }
   }
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sums[wave][j * 64 + lane] = acc[j];
@@ -333,12 +350,13 @@ bool packed8(int64_t H, int64_t ld, const void* p, const void* q) {
 constexpr int64_t MAX_THREADS = (int64_t)1 << 32;
 
 struct BwdLayout {
-  int64_t runs, start, order, partial, bytes;
+  int64_t runs, start, order, over, partial, bytes;
   BwdLayout(int64_t T, int64_t H, int64_t V) {
     runs = ceil_div_i64(T, RUN);
     start = 0;
     order = round_up_i64((V + 1) * 4, 256);
-    partial = order + round_up_i64(T * 4, 256);
+    over = order + round_up_i64(T * 4, 256);
+    partial = over + round_up_i64(runs * 4, 256);
     bytes = partial + runs * 2 * H * 4;
   }
 };
@@ -405,12 +423,13 @@ int areal_embedding_bwd(const void* grad, int grad_dtype, const int64_t* ids, in
         a.partial = (float*)(ws + l.partial);
         a.T = (int)T; a.V = (int)V; a.H = (int)H; a.scale = scale;
         const int64_t slabs = ceil_div_i64(H, 64 * VEC), sum_blocks = ceil_div_i64(l.runs * slabs, 4);
-        const int64_t fill_blocks = accumulate ? 0 : ceil_div_i64(V, 4 * FILL_ROWS);
         const int64_t range = std::min<int64_t>(ceil_div_i64(V, 256), RANGE_MAX);
         const int64_t ranges = ceil_div_i64(V, range);
+        const int64_t fill_blocks = accumulate ? 0 : ceil_div_i64(V, 4 * FILL_ROWS);
         if ((sum_blocks + fill_blocks) * 256 >= MAX_THREADS || l.runs * slabs * 64 * JOIN_WAVES >= MAX_THREADS ||
             ranges * 64 * SORT_WAVES >= MAX_THREADS)
           return AREAL_ERR_UNSUPPORTED;
+        a.over = (int*)(ws + l.over);
         a.runs = (unsigned)l.runs; a.slabs = (unsigned)slabs; a.sum_blocks = (unsigned)sum_blocks;
         hipLaunchKernelGGL(embedding_order_kernel, dim3((unsigned)ranges), dim3(64 * SORT_WAVES),
                            (size_t)range * SORT_WAVES * 4, stream, ids, (int)T, (int)V, (int)range, padding_idx,
