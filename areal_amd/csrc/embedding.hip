@@ -43,7 +43,7 @@ DEVI void load_pack(const T* p, Pack<T, VEC>& o) {
     __builtin_memcpy(&o, raw, sizeof(o));
   }
 }
-template <typename T, int VEC>
+template <typename T, int VEC, bool NT = false>
 DEVI void store_pack(T* p, const Pack<T, VEC>& o) {
   if constexpr (VEC == 1) {
     *p = o.v[0];
@@ -52,17 +52,24 @@ DEVI void store_pack(T* p, const Pack<T, VEC>& o) {
     u32x4 raw[N];
     __builtin_memcpy(raw, &o, sizeof(o));
 #pragma unroll
-    for (int i = 0; i < N; ++i) ((u32x4*)p)[i] = raw[i];
+    for (int i = 0; i < N; ++i) {
+      if (NT) __builtin_nontemporal_store(raw[i], (u32x4*)p + i);
+      else ((u32x4*)p)[i] = raw[i];
+    }
   }
 }
 
 // Loads that run ahead of their use have no condition: behind the row's or the list's end they repeat its first or last
-// piece. (Behind a branch each, the compiler waits for the one before: the 32 rows of embedding_sum_kernel one by one, 127
-// us for 32768 x 4096 bf16 that take 60.)
+// piece. (Behind a branch each, the compiler waits for the one before: the rows of embedding_sum_kernel one by one, 28 us
+// for 509 x 896 bf16 that take 14.)
 
 // A wave takes ROW_PACKS packs per lane of one row: all loads before the first store.
-constexpr int ROW_PACKS = 4;
-template <typename W, typename O, int VEC>
+// Two packs: 64 x 4096 bf16 3.1 us, with four 3.4, with eight 4.2; 32768 x 4096 alike.
+// NT: outputs that the memory-side cache of 256 MB does not hold for their reader are stored with the non-temporal hint:
+// 32768 x 4096 bf16 77 us, 93 without.
+constexpr int ROW_PACKS = 2;
+constexpr int64_t NT_BYTES = (int64_t)256 << 20;
+template <typename W, typename O, int VEC, bool NT>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const W* __restrict__ weight, int64_t ldw,
                                                             const int64_t* __restrict__ ids, unsigned units,
                                                             unsigned parts, int V, int H, float scale,
@@ -88,22 +95,153 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const W* __restrict_
       Pack<O, VEC> y;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) y.v[j] = narrow1<O>(in ? widen1<W>(x[i].v[j]) * scale : 0.f);
-      store_pack<O, VEC>(dst + at, y);
+      store_pack<O, VEC, NT>(dst + at, y);
     }
   }
 }
 
 // ---- the order of the tokens by id ----
+// order[start[v] .. start[v + 1]): the tokens of id v, ascending. A workgroup places those of a range of ids, a wave of it one
+// run of tokens, so that places follow from the counts of the waves before it. Up to FEW_TOKENS it reads all ids (one
+// launch, but every workgroup looks at every token: 16384 took 29 us, 32768 53); beyond, two launches deal the tokens out to
+// the ranges first, in their order.
 constexpr int SORT_WAVES = 16;
 constexpr int RANGE_BITS = 10;
-constexpr int RANGE_MAX = 768;  // ids of a workgroup: 16 waves' counts of them take 48 KB of LDS
+constexpr int RANGE_MAX = 768;     // ids of a workgroup: 16 waves' counts of them take 48 KB of LDS
+constexpr int MAX_RANGES = 960;    // that tokens are dealt out to
 constexpr int SORT_UNROLL = 8;
+constexpr int64_t FEW_TOKENS = 8192;
+constexpr uint32_t NONE = 0xffffffffu;  // for ids that count nowhere (V is at most 2^31 - 2)
 
-// order[start[v] .. start[v + 1]): the tokens of id v, ascending. A workgroup reads all ids twice (from the L2 of its
-// XCD) and places those of its range; how many tokens have lower ids, it counts on the way. A wave takes one run of
-// tokens, so that places follow from the counts of the waves before it.
+DEVI uint32_t id_or_none(uint2 raw, int V, uint32_t padding) {
+  return raw.y == 0 && raw.x < (uint32_t)V && raw.x != padding ? raw.x : NONE;
+}
+// The place of this lane's `key` (below 2^RANGE_BITS where `in`), which places[key] counts on: lanes of one key in their
+// order. By a wave whose own `places` are.
+DEVI int next_place(uint32_t key, bool in, volatile int* places, int lane) {
+  const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
+  if (all == 0) return 0;
+  // the lanes with this lane's key: those that agree with it in every bit (a hot range has a dozen ids among 64 tokens: one
+  // id at a time took 85 us for 32768 tokens, this 53)
+  unsigned long long same = all;
+#pragma unroll
+  for (int bit = 0; bit < RANGE_BITS; ++bit) {
+    const unsigned long long set = __builtin_amdgcn_ballot_w64(key >> bit & 1);
+    same &= key >> bit & 1 ? set : ~set;
+  }
+  int to = 0;
+  if (in) {
+    const int before = __popcll(same & ((1ull << lane) - 1));
+    to = places[key] + before;
+    if (before == 0) places[key] = to + __popcll(same);
+  }
+  return to;
+}
+// f(position, value) for [begin, end), 64 a step by a wave; value = load(position), `missing` behind the end.
+template <class T, class L, class F>
+DEVI void sweep_tokens(int64_t begin, int64_t end, int lane, T missing, L load, F f) {
+  for (int64_t t = begin; t < end; t += SORT_UNROLL * 64) {
+    T v[SORT_UNROLL];
+#pragma unroll
+    for (int i = 0; i < SORT_UNROLL; ++i) v[i] = load(min(t + i * 64 + lane, end - 1));
+#pragma unroll
+    for (int i = 0; i < SORT_UNROLL; ++i) {
+      const int64_t at = t + i * 64 + lane;
+      f((int)at, at < end ? v[i] : missing);
+    }
+  }
+}
+// The wave's run of [0, n): whole steps of 64.
+DEVI void wave_run(int64_t n, int wave, int64_t& begin, int64_t& end) {
+  const int64_t run = (n + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64;
+  begin = min((int64_t)wave * run, n);
+  end = min(begin + run, n);
+}
+
+// What the tokens are dealt out with, for `chunks` runs of `chunk` tokens.
+struct Deal {
+  int* counts;       // [chunks][ranges]
+  int* range_start;  // [ranges + 1]
+  uint32_t* id;      // [T]: ids and tokens, by range
+  int* token;
+  int64_t chunk;
+  int chunks, ranges, range;
+};
+__global__ __launch_bounds__(64 * SORT_WAVES) void embedding_count_kernel(const int64_t* __restrict__ ids, int T, int V,
+                                                                          int64_t padding_idx, Deal d) {
+  __shared__ int counts[MAX_RANGES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int i = tid; i < d.ranges; i += 64 * SORT_WAVES) counts[i] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * d.chunk, n = min(d.chunk, T - first);
+  const uint32_t padding = padding_idx < 0 ? NONE : (uint32_t)padding_idx;
+  int64_t begin, end;
+  wave_run(n, wave, begin, end);
+  sweep_tokens(begin, end, lane, make_uint2(NONE, NONE), [&](int64_t t) { return ((const uint2*)ids)[first + t]; },
+               [&](int, uint2 raw) {
+                 const uint32_t id = id_or_none(raw, V, padding);
+                 if (id != NONE) atomicAdd(&counts[id / (uint32_t)d.range], 1);
+               });
+  __syncthreads();
+  for (int i = tid; i < d.ranges; i += 64 * SORT_WAVES) d.counts[(int64_t)blockIdx.x * d.ranges + i] = counts[i];
+}
+__global__ __launch_bounds__(64 * SORT_WAVES) void embedding_deal_kernel(const int64_t* __restrict__ ids, int T, int V,
+                                                                         int64_t padding_idx, Deal d) {
+  extern __shared__ int places[];  // [SORT_WAVES][ranges]
+  __shared__ int part[SORT_WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = blockIdx.x;
+  for (int i = tid; i < SORT_WAVES * d.ranges; i += 64 * SORT_WAVES) places[i] = 0;
+  // thread r: tokens of range r, and of them those in the chunks before this one (MAX_RANGES threads)
+  int total = 0, before = 0;
+  if (tid < d.ranges)
+    for (int c = 0; c < d.chunks; ++c) {
+      const int n = d.counts[(int64_t)c * d.ranges + tid];
+      total += n;
+      before += c < chunk ? n : 0;
+    }
+  const int incl = wave_inclusive_scan(total, 0, [](int x, int y) { return x + y; });
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int at = incl - total;
+  for (int w = 0; w < wave; ++w) at += part[w];
+  if (chunk == 0 && tid < d.ranges) {
+    d.range_start[tid] = at;
+    if (tid == d.ranges - 1) d.range_start[d.ranges] = at + total;
+  }
+  at += before;
+  const int64_t first = (int64_t)chunk * d.chunk, n = min(d.chunk, T - first);
+  const uint32_t padding = padding_idx < 0 ? NONE : (uint32_t)padding_idx;
+  int* const own = places + wave * d.ranges;
+  int64_t begin, end;
+  wave_run(n, wave, begin, end);
+  auto sweep = [&](auto f) {
+    sweep_tokens(begin, end, lane, make_uint2(NONE, NONE), [&](int64_t t) { return ((const uint2*)ids)[first + t]; },
+                 [&](int t, uint2 raw) { f(t, id_or_none(raw, V, padding)); });
+  };
+  sweep([&](int, uint32_t id) {
+    if (id != NONE) atomicAdd(&own[id / (uint32_t)d.range], 1);
+  });
+  __syncthreads();
+  if (tid < d.ranges)
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const int c = places[w * d.ranges + tid];
+      places[w * d.ranges + tid] = at;
+      at += c;
+    }
+  __syncthreads();
+  sweep([&](int t, uint32_t id) {
+    const bool in = id != NONE;
+    const int to = next_place(in ? id / (uint32_t)d.range : 0, in, own, lane);
+    if (in) {
+      d.id[to] = id;
+      d.token[to] = (int)(first + t);
+    }
+  });
+}
+
+template <bool DEALT>
 __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const int64_t* __restrict__ ids, int T, int V,
-                                                                          int range, int64_t padding_idx,
+                                                                          int range, int64_t padding_idx, Deal d,
                                                                           int* __restrict__ start,
                                                                           int* __restrict__ order) {
   extern __shared__ int counts[];  // [SORT_WAVES][range]
@@ -114,29 +252,22 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const 
   for (int i = tid; i < SORT_WAVES * range; i += 64 * SORT_WAVES) counts[i] = 0;
   __syncthreads();
   int* const own = counts + wave * range;
-  // an odd number of 512-byte steps: with runs of 16 KB all waves of all workgroups read the same channel of an L2
-  const int run = (int)(((int64_t)T + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) | 1) * 64;
-  const int64_t t0 = min((int64_t)wave * run, (int64_t)T), t1 = min(t0 + run, (int64_t)T);
-  // f(token, id - lo as an unsigned number): below n for ids of the range, above -lo for lower ones; SORT_UNROLL x 64
-  // tokens at a time. (NONE, of ids that count nowhere, is neither: V is at most 2^31 - 2.)
-  constexpr uint32_t NONE = 0xffffffffu;
+  const int first = DEALT ? d.range_start[blockIdx.x] : 0;
   const uint32_t padding = padding_idx < 0 ? NONE : (uint32_t)padding_idx;
+  int64_t begin, end;
+  wave_run(DEALT ? d.range_start[blockIdx.x + 1] - first : T, wave, begin, end);
+  // f(token, id): the range's tokens and ids, or all
   auto sweep = [&](auto f) {
-    for (int64_t t = t0; t < t1; t += SORT_UNROLL * 64) {
-      uint2 raw[SORT_UNROLL];
-#pragma unroll
-      for (int i = 0; i < SORT_UNROLL; ++i) {
-        const int64_t at = t + i * 64 + lane;
-        raw[i] = at < t1 ? ((const uint2*)ids)[at] : make_uint2(NONE, NONE);
-      }
-#pragma unroll
-      for (int i = 0; i < SORT_UNROLL; ++i) {
-        const uint32_t id = raw[i].y == 0 && raw[i].x < (uint32_t)V && raw[i].x != padding ? raw[i].x : NONE;
-        f((int)(t + i * 64 + lane), id);
-      }
+    if constexpr (DEALT) {
+      sweep_tokens(begin, end, lane, make_uint2(NONE, 0), [&](int64_t t) {
+        return make_uint2(d.id[first + t], (uint32_t)d.token[first + t]);
+      }, [&](int, uint2 v) { f((int)v.y, v.x); });
+    } else {
+      sweep_tokens(begin, end, lane, make_uint2(NONE, NONE), [&](int64_t t) { return ((const uint2*)ids)[t]; },
+                   [&](int t, uint2 raw) { f(t, id_or_none(raw, V, padding)); });
     }
   };
-  int below = 0;
+  int below = 0;  // tokens of lower ids (of those dealt out, `first` are)
   sweep([&](int, uint32_t id) {
     below += id < (uint32_t)lo;
     if (id - (uint32_t)lo < (uint32_t)n) atomicAdd(&own[id - (uint32_t)lo], 1);
@@ -144,7 +275,7 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const 
   below = wave_sum(below);
   if (lane == 0) below_of[wave] = below;
   __syncthreads();
-  int base = 0;
+  int base = first;
 #pragma unroll
   for (int w = 0; w < SORT_WAVES; ++w) base += below_of[w];
   // thread v: id lo + v (range <= threads)
@@ -167,25 +298,11 @@ __global__ __launch_bounds__(64 * SORT_WAVES) void embedding_order_kernel(const 
     }
   }
   __syncthreads();
-  volatile int* const places = own;  // of this wave alone from here on
   sweep([&](int t, uint32_t id) {
     const uint32_t rel = id - (uint32_t)lo;
     const bool in = rel < (uint32_t)n;
-    const unsigned long long all = __builtin_amdgcn_ballot_w64(in);
-    if (all == 0) return;
-    // the lanes with this lane's id: those that agree with it in every bit (a hot range has a dozen ids among 64 tokens,
-    // one id at a time took 37 us of 85 at 32 Ki tokens)
-    unsigned long long same = all;
-#pragma unroll
-    for (int bit = 0; bit < RANGE_BITS; ++bit) {
-      const unsigned long long set = __builtin_amdgcn_ballot_w64(rel >> bit & 1);
-      same &= rel >> bit & 1 ? set : ~set;
-    }
-    if (in) {
-      const int to = places[rel], before = __popcll(same & ((1ull << lane) - 1));
-      order[to + before] = t;
-      if (before == 0) places[rel] = to + __popcll(same);
-    }
+    const int to = next_place(rel, in, own, lane);
+    if (in) order[to] = t;
   });
 }
 
@@ -350,14 +467,23 @@ bool packed8(int64_t H, int64_t ld, const void* p, const void* q) {
 constexpr int64_t MAX_THREADS = (int64_t)1 << 32;
 
 struct BwdLayout {
-  int64_t runs, start, order, over, partial, bytes;
+  int64_t runs, range, ranges, chunk, chunks, start, order, over, partial, counts, range_start, deal_id, deal_token, bytes;
   BwdLayout(int64_t T, int64_t H, int64_t V) {
     runs = ceil_div_i64(T, RUN);
+    range = std::min<int64_t>(ceil_div_i64(V, 256), RANGE_MAX);
+    ranges = ceil_div_i64(V, range);
+    // runs of tokens that are dealt out to the ranges by one workgroup each; 0: they are not
+    chunk = std::max<int64_t>(round_up_i64(ceil_div_i64(T, 128), 1024), 2048);
+    chunks = T > FEW_TOKENS && ranges <= MAX_RANGES ? ceil_div_i64(T, chunk) : 0;
     start = 0;
     order = round_up_i64((V + 1) * 4, 256);
     over = order + round_up_i64(T * 4, 256);
     partial = over + round_up_i64(runs * 4, 256);
-    bytes = partial + runs * 2 * H * 4;
+    counts = round_up_i64(partial + runs * 2 * H * 4, 256);
+    range_start = round_up_i64(counts + chunks * ranges * 4, 256);
+    deal_id = round_up_i64(range_start + (chunks > 0 ? ranges + 1 : 0) * 4, 256);
+    deal_token = round_up_i64(deal_id + (chunks > 0 ? T : 0) * 4, 256);
+    bytes = deal_token + (chunks > 0 ? T : 0) * 4;
   }
 };
 
@@ -376,18 +502,19 @@ int areal_embedding_fwd(const void* weight, int weight_dtype, int64_t ldw, const
     return with_type(out_dtype, [&](auto o) {
       using W = decltype(w);
       using O = decltype(o);
-      auto launch = [&](auto vec) -> int {
+      auto launch = [&](auto vec, auto nt) -> int {
         constexpr int VEC = decltype(vec)::value;
         const int64_t parts = ceil_div_i64(H, 64 * VEC * ROW_PACKS), units = T * parts;
         if (units * 64 >= MAX_THREADS) return AREAL_ERR_UNSUPPORTED;
-        hipLaunchKernelGGL((embedding_fwd_kernel<W, O, VEC>), dim3((unsigned)ceil_div_i64(units, 4)), dim3(256), 0,
+        hipLaunchKernelGGL((embedding_fwd_kernel<W, O, VEC, decltype(nt)::value>), dim3((unsigned)ceil_div_i64(units, 4)), dim3(256), 0,
                            stream, (const W*)weight, ldw, ids, (unsigned)units, (unsigned)parts, (int)V, (int)H, scale,
                            (O*)out);
         AREAL_CHECK_LAUNCH();
         return AREAL_OK;
       };
-      return packed8(H, ldw, weight, out) ? launch(std::integral_constant<int, 8>{})
-                                          : launch(std::integral_constant<int, 1>{});
+      if (!packed8(H, ldw, weight, out)) return launch(std::integral_constant<int, 1>{}, std::false_type{});
+      const std::integral_constant<int, 8> eight;
+      return T * H * (int64_t)sizeof(O) >= NT_BYTES ? launch(eight, std::true_type{}) : launch(eight, std::false_type{});
     });
   });
 }
@@ -423,17 +550,29 @@ int areal_embedding_bwd(const void* grad, int grad_dtype, const int64_t* ids, in
         a.partial = (float*)(ws + l.partial);
         a.T = (int)T; a.V = (int)V; a.H = (int)H; a.scale = scale;
         const int64_t slabs = ceil_div_i64(H, 64 * VEC), sum_blocks = ceil_div_i64(l.runs * slabs, 4);
-        const int64_t range = std::min<int64_t>(ceil_div_i64(V, 256), RANGE_MAX);
-        const int64_t ranges = ceil_div_i64(V, range);
         const int64_t fill_blocks = accumulate ? 0 : ceil_div_i64(V, 4 * FILL_ROWS);
         if ((sum_blocks + fill_blocks) * 256 >= MAX_THREADS || l.runs * slabs * 64 * JOIN_WAVES >= MAX_THREADS ||
-            ranges * 64 * SORT_WAVES >= MAX_THREADS)
+            l.ranges * 64 * SORT_WAVES >= MAX_THREADS)
           return AREAL_ERR_UNSUPPORTED;
         a.over = (int*)(ws + l.over);
         a.runs = (unsigned)l.runs; a.slabs = (unsigned)slabs; a.sum_blocks = (unsigned)sum_blocks;
-        hipLaunchKernelGGL(embedding_order_kernel, dim3((unsigned)ranges), dim3(64 * SORT_WAVES),
-                           (size_t)range * SORT_WAVES * 4, stream, ids, (int)T, (int)V, (int)range, padding_idx,
-                           (int*)(ws + l.start), (int*)(ws + l.order));
+        const Deal d{(int*)(ws + l.counts), (int*)(ws + l.range_start), (uint32_t*)(ws + l.deal_id),
+                     (int*)(ws + l.deal_token), l.chunk, (int)l.chunks, (int)l.ranges, (int)l.range};
+        const dim3 threads(64 * SORT_WAVES);
+        const size_t lds = (size_t)l.range * SORT_WAVES * 4;
+        int* const start = (int*)(ws + l.start);
+        int* const order = (int*)(ws + l.order);
+        if (l.chunks > 0) {
+          hipLaunchKernelGGL(embedding_count_kernel, dim3((unsigned)l.chunks), threads, 0, stream, ids, (int)T, (int)V,
+                             padding_idx, d);
+          hipLaunchKernelGGL(embedding_deal_kernel, dim3((unsigned)l.chunks), threads, (size_t)l.ranges * SORT_WAVES * 4,
+                             stream, ids, (int)T, (int)V, padding_idx, d);
+          hipLaunchKernelGGL((embedding_order_kernel<true>), dim3((unsigned)l.ranges), threads, lds, stream, ids, (int)T,
+                             (int)V, (int)l.range, padding_idx, d, start, order);
+        } else {
+          hipLaunchKernelGGL((embedding_order_kernel<false>), dim3((unsigned)l.ranges), threads, lds, stream, ids, (int)T,
+                             (int)V, (int)l.range, padding_idx, d, start, order);
+        }
         AREAL_CHECK_LAUNCH();
         auto sums = [&](auto add) {
           constexpr bool ADD = decltype(add)::value;
