@@ -24,6 +24,7 @@ constexpr float LN2_F = 0.6931471805599453f;
 // with unaligned access enabled: still one 16-byte instruction); stores are aligned by their caller.
 template <typename T> struct Elem;
 template <> struct Elem<float> {
+  typedef f32x4 Reg;
   typedef f32x4 Vec __attribute__((aligned(4)));
   static constexpr int VEC = 4;
   static DEVI float load(const float* p) { return *p; }
@@ -39,6 +40,7 @@ template <> struct Elem<float> {
   }
 };
 template <> struct Elem<u16> {  // bf16 bit patterns
+  typedef u32x4 Reg;
   typedef u32x4 Vec __attribute__((aligned(2)));
   static constexpr int VEC = 8;
   static DEVI float load(const u16* p) { return bf16_bits_to_f32(*p); }
@@ -67,6 +69,7 @@ template <> struct Elem<u16> {  // bf16 bit patterns
 
 template <> struct Elem<_Float16> {
   typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  typedef f16x8 Reg;
   typedef f16x8 Vec __attribute__((aligned(2)));
   static constexpr int VEC = 8;
   static DEVI float load(const _Float16* p) { return (float)*p; }
@@ -350,20 +353,6 @@ constexpr int KEPT_STEP = 2048, KEPT_UNIT = 8, KEPT_STEPS = 4;
 // Exponents are held above this: a kept logit of -inf then adds 0 to sums of t * 2^t (a NaN stays one).
 constexpr float KEPT_LOWEST = -160.f;
 
-template <typename T>
-DEVI void load_unit(const T* x, int at, int V, float (&z)[KEPT_UNIT]) {
-  constexpr int VEC = Elem<T>::VEC;
-  if (at + KEPT_UNIT <= V) {
-    typename Elem<T>::Vec v[KEPT_UNIT / VEC];
-#pragma unroll
-    for (int i = 0; i < KEPT_UNIT / VEC; ++i) v[i] = *(const typename Elem<T>::Vec*)(x + at + i * VEC);
-#pragma unroll
-    for (int i = 0; i < KEPT_UNIT / VEC; ++i) Elem<T>::widen(v[i], z + i * VEC);
-  } else {
-#pragma unroll
-    for (int i = 0; i < KEPT_UNIT; ++i) z[i] = at + i < V ? Elem<T>::load(x + at + i) : neg_inf();
-  }
-}
 // Word `w` of a row; bits behind the vocabulary do not count.
 DEVI uint32_t kept_word(const uint32_t* kept, int w, int V) {
   if (w * 32 >= V) return 0;
@@ -374,15 +363,54 @@ DEVI uint32_t kept_word(const uint32_t* kept, int w, int V) {
 DEVI uint32_t kept_byte(uint32_t word, int step, int lane) {
   return (__shfl((int)word, step * 16 + (lane >> 2), 64) >> ((lane & 3) * 8)) & 0xff;
 }
+// The bytes of the 256 units from token c on, and the logits of those that have a bit, for c + KEPT_STEP <= V. All loads are
+// under way together: lanes without a bit read the first unit (behind a branch each, a load waits for the one before).
+template <typename T>
+struct KeptRaw {
+  typename Elem<T>::Reg v[KEPT_STEPS][KEPT_UNIT / Elem<T>::VEC];
+  uint32_t b[KEPT_STEPS];
+  DEVI void load(const T* x, int c, uint32_t word, int lane) {
+#pragma unroll
+    for (int i = 0; i < KEPT_STEPS; ++i) {
+      b[i] = kept_byte(word, i, lane);
+      const T* const from = x + c + (b[i] != 0 ? (i * 64 + lane) * KEPT_UNIT : 0);
+#pragma unroll
+      for (int k = 0; k < KEPT_UNIT / Elem<T>::VEC; ++k) v[i][k] = ((const typename Elem<T>::Vec*)from)[k];
+    }
+  }
+  DEVI void widen(float (&z)[KEPT_STEPS][KEPT_UNIT]) const {
+#pragma unroll
+    for (int i = 0; i < KEPT_STEPS; ++i) {
+#pragma unroll
+      for (int k = 0; k < KEPT_UNIT / Elem<T>::VEC; ++k) Elem<T>::widen(v[i][k], z[i] + k * Elem<T>::VEC);
+    }
+  }
+};
+// The same for the last tokens of a row.
+template <typename T>
+DEVI void load_kept_end(const T* x, int c, int V, uint32_t word, int lane, uint32_t (&b)[KEPT_STEPS],
+                        float (&z)[KEPT_STEPS][KEPT_UNIT]) {
+#pragma unroll
+  for (int i = 0; i < KEPT_STEPS; ++i) {
+    b[i] = kept_byte(word, i, lane);
+    const int at = c + (i * 64 + lane) * KEPT_UNIT;
+#pragma unroll
+    for (int j = 0; j < KEPT_UNIT; ++j) z[i][j] = b[i] != 0 && at + j < V ? Elem<T>::load(x + at + j) : neg_inf();
+  }
+}
 DEVI bool kept_at(const uint32_t* kept, int64_t token) { return kept[token >> 5] >> (token & 31) & 1; }
 
-DEVI void online_add_kept(Online& st, const float (&x)[KEPT_UNIT], uint32_t bits, float c2) {
-  float z[KEPT_UNIT], xm = neg_inf();
+// Adds the logits of a lane's units whose bits are set. ALL: all are.
+template <bool ALL>
+DEVI void online_add_kept(Online& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], float c2) {
+  float xm = neg_inf();
 #pragma unroll
-  for (int i = 0; i < KEPT_UNIT; ++i) {
-    z[i] = bits >> i & 1 ? x[i] : neg_inf();
-    xm = fmaxf(xm, z[i]);
-  }
+  for (int k = 0; k < KEPT_STEPS; ++k)
+#pragma unroll
+    for (int i = 0; i < KEPT_UNIT; ++i) {
+      if (!ALL) z[k][i] = b[k] >> i & 1 ? z[k][i] : neg_inf();
+      xm = fmaxf(xm, z[k][i]);
+    }
   const float vm = xm * c2;
   if (vm > st.m) {
     if (st.m > neg_inf()) {
@@ -394,14 +422,21 @@ DEVI void online_add_kept(Online& st, const float (&x)[KEPT_UNIT], uint32_t bits
   }
   const float m = st.m > neg_inf() ? st.m : 0.f;
 #pragma unroll
-  for (int i = 0; i < KEPT_UNIT; ++i) {
-    const float t = stat_max(fmaf(z[i], c2, -m), KEPT_LOWEST);
-    const float e = fast_exp2(t);
-    st.s += e;
-    st.q = fmaf(t, e, st.q);
+  for (int k = 0; k < KEPT_STEPS; ++k) {
+    if (!ALL && __builtin_amdgcn_ballot_w64(b[k] != 0) == 0) continue;
+#pragma unroll
+    for (int i = 0; i < KEPT_UNIT; ++i) {
+      const float t = stat_max(fmaf(z[k][i], c2, -m), KEPT_LOWEST);
+      const float e = fast_exp2(t);
+      st.s += e;
+      st.q = fmaf(t, e, st.q);
+    }
   }
 }
 
+// Bound by the latency of its scattered reads: 2048 x 151936 bf16, a quarter of the rows kept whole, reads 230 MB in 83 us
+// with blocks of 256 threads, 90 with 512, 116 with 1024 (99 without the next step's loads under way, 114 with one wait
+// per load); 93 x 50257 fp32 11.0, 8.4 and 11.4 us.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__ logits, int64_t ld,
                                                            const int64_t* __restrict__ labels,
@@ -416,28 +451,37 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float c2 = inv_temp * LOG2E_F;
   Online st{neg_inf(), 0.f, 0.f};
-  for (int64_t c0 = (int64_t)wave * KEPT_STEP; c0 < V; c0 += (int64_t)AHEAD * WAVES * KEPT_STEP) {
+  auto add = [&](float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], uint32_t word) {
+    if (__builtin_amdgcn_ballot_w64(word == 0xffffffffu) == ~0ull) online_add_kept<true>(st, z, b, c2);
+    else if (__builtin_amdgcn_ballot_w64(word != 0) != 0) online_add_kept<false>(st, z, b, c2);
+  };
+  const int whole = V / KEPT_STEP;  // steps without the row's end; a wave takes every WAVES-th
+  for (int s0 = wave; s0 < whole; s0 += AHEAD * WAVES) {
     uint32_t words[AHEAD];
+    int step[AHEAD];
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const int64_t c = c0 + (int64_t)a * WAVES * KEPT_STEP;
-      words[a] = c < V ? kept_word(bits, (int)(c / 32) + lane, V) : 0;
+      step[a] = min(s0 + a * WAVES, whole - 1);
+      const uint32_t word = bits[step[a] * 64 + lane];
+      words[a] = s0 + a * WAVES < whole ? word : 0;
     }
+    KeptRaw<T> raw[2];  // the next step's logits are under way
+    raw[0].load(x, step[0] * KEPT_STEP, words[0], lane);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      if (__builtin_amdgcn_ballot_w64(words[a] != 0) == 0) continue;
-      const int c = (int)(c0 + (int64_t)a * WAVES * KEPT_STEP);
+      if (a + 1 < AHEAD) raw[(a + 1) & 1].load(x, step[a + 1] * KEPT_STEP, words[a + 1], lane);
       float z[KEPT_STEPS][KEPT_UNIT];
-      uint32_t b[KEPT_STEPS];
-#pragma unroll
-      for (int i = 0; i < KEPT_STEPS; ++i) {
-        b[i] = kept_byte(words[a], i, lane);
-        if (b[i] != 0) load_unit<T>(x, c + (i * 64 + lane) * KEPT_UNIT, V, z[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < KEPT_STEPS; ++i)
-        if (b[i] != 0) online_add_kept(st, z[i], b[i], c2);
+      raw[a & 1].widen(z);
+      add(z, raw[a & 1].b, words[a]);
     }
+  }
+  if (whole * KEPT_STEP < V && wave == whole % WAVES) {
+    const int c = whole * KEPT_STEP;
+    const uint32_t word = kept_word(bits, c / 32 + lane, V);
+    float z[KEPT_STEPS][KEPT_UNIT];
+    uint32_t b[KEPT_STEPS];
+    load_kept_end<T>(x, c, V, word, lane, b, z);
+    add(z, b, word);
   }
   const Online r = block_merge(st, smem);
   if (threadIdx.x == 0) {
@@ -460,7 +504,8 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
   }
 }
 
-// Block (row, part): part_steps runs of KEPT_STEP tokens.
+// Block (row, part): part_steps runs of KEPT_STEP tokens. Bound by HBM: 2048 x 151936 bf16 moves 860 MB in 188 us, 622 of them
+// written.
 constexpr int KEPT_BWD_WAVES = 4;
 template <typename T, bool ENT>
 __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
@@ -492,10 +537,25 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
     const uint32_t word = none ? 0 : kept_word(bits, c / 32 + lane, V);
     float z[KEPT_STEPS][KEPT_UNIT];
     uint32_t b[KEPT_STEPS];
+    if (__builtin_amdgcn_ballot_w64(word != 0) == 0 && c + KEPT_STEP <= V) {  // nothing kept
 #pragma unroll
-    for (int i = 0; i < KEPT_STEPS; ++i) {
-      b[i] = kept_byte(word, i, lane);
-      if (b[i] != 0) load_unit<T>(x, c + (i * 64 + lane) * KEPT_UNIT, V, z[i]);
+      for (int j = 0; j < KEPT_UNIT; ++j) z[0][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i) {
+#pragma unroll
+        for (int j = 0; j < KEPT_UNIT / VEC; ++j)
+          Elem<T>::storeu(d + c + (i * 64 + lane) * KEPT_UNIT + j * VEC, z[0] + j * VEC);
+      }
+      continue;
+    }
+    if (c + KEPT_STEP <= V) {
+      KeptRaw<T> raw;
+      raw.load(x, c, word, lane);
+      raw.widen(z);
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i) b[i] = raw.b[i];
+    } else {
+      load_kept_end<T>(x, c, V, word, lane, b, z);
     }
 #pragma unroll
     for (int i = 0; i < KEPT_STEPS; ++i) {
@@ -536,7 +596,7 @@ int launch_kept_fwd(const void* logits, int64_t ld, const int64_t* labels, const
                        labels, kept, kept_ld, (int)V, inv_temp, lp, ent, lse2);
   };
   if (N < FWD_FEW_ROWS)
-    launch(std::integral_constant<int, 1024>{});
+    launch(std::integral_constant<int, 512>{});
   else
     launch(std::integral_constant<int, 256>{});
   AREAL_CHECK_LAUNCH();
