@@ -504,12 +504,16 @@ int areal_embedding_fwd(const void* weight, int weight_dtype, int64_t ldw, const
       using O = decltype(o);
       auto launch = [&](auto vec, auto nt) -> int {
         constexpr int VEC = decltype(vec)::value;
-        const int64_t parts = ceil_div_i64(H, 64 * VEC * ROW_PACKS), units = T * parts;
-        if (units * 64 >= MAX_THREADS) return AREAL_ERR_UNSUPPORTED;
-        hipLaunchKernelGGL((embedding_fwd_kernel<W, O, VEC, decltype(nt)::value>), dim3((unsigned)ceil_div_i64(units, 4)), dim3(256), 0,
-                           stream, (const W*)weight, ldw, ids, (unsigned)units, (unsigned)parts, (int)V, (int)H, scale,
-                           (O*)out);
-        AREAL_CHECK_LAUNCH();
+        const int64_t parts = ceil_div_i64(H, 64 * VEC * ROW_PACKS);
+        const int64_t most = std::max<int64_t>((MAX_THREADS / 64 - 4) / parts, 1);  // tokens of a launch
+        if (parts >= MAX_THREADS / 64 - 4) return AREAL_ERR_UNSUPPORTED;
+        for (int64_t t0 = 0; t0 < T; t0 += most) {
+          const int64_t units = std::min(most, T - t0) * parts;
+          hipLaunchKernelGGL((embedding_fwd_kernel<W, O, VEC, decltype(nt)::value>),
+                             dim3((unsigned)ceil_div_i64(units, 4)), dim3(256), 0, stream, (const W*)weight, ldw, ids + t0,
+                             (unsigned)units, (unsigned)parts, (int)V, (int)H, scale, (O*)out + t0 * H);
+          AREAL_CHECK_LAUNCH();
+        }
         return AREAL_OK;
       };
       if (!packed8(H, ldw, weight, out)) return launch(std::integral_constant<int, 1>{}, std::false_type{});

@@ -21,8 +21,12 @@ constexpr int SUBS = 16;             // maxima kept of a segment where top-k ask
 constexpr int MAX_SEGS = 4096;       // vocabularies up to 4 Mi
 constexpr int FEW_SEGS = 512;        // up to 512 Ki
 constexpr unsigned MANY_SEGS = 16384;  // from here a wave takes four segments of the first pass
+// Up to here a row has 1024 threads, beyond 512, two workgroups a CU: with top-p 0.9 400 x 151936 bf16 212 and 184 us.
 constexpr int64_t FEW_ROWS = 256;
-constexpr int64_t SPREAD_ROWS = 128;   // up to here rows with many candidates are spread over workgroups
+// Up to so many rows of at least so many segments the ones with many candidates are spread over workgroups: with top-p 0.9
+// 1 x 151936 bf16 takes 52 us spread and 80 by one workgroup, 64 rows 80 and 91, 128 rows 106 and 101; 8 x 50257 51 and 52,
+// 8 x 32000 60 and 42.
+constexpr int64_t SPREAD_ROWS = 64, SPREAD_SEGS = 80;
 constexpr int LIST = 4096;           // candidates held in LDS
 constexpr double LOG2E = 1.4426950408889634;
 
@@ -363,6 +367,16 @@ struct RowShared {
   double target;
 };
 constexpr int NO_INDEX = 0x7fffffff;
+// *to = the lowest (highest) v of the workgroup, where v rises with the thread from the first on that has one (NO_INDEX,
+// -1: has none): one atomic a wave, as 1024 on one word take 14,000 clocks.
+DEVI void lowest_of(int v, int* to) {
+  const unsigned long long has = __builtin_amdgcn_ballot_w64(v != NO_INDEX);
+  if (has != 0 && (int)(threadIdx.x & 63) == __builtin_ctzll(has)) atomicMin(to, v);
+}
+DEVI void highest_of(int v, int* to) {
+  const unsigned long long has = __builtin_amdgcn_ballot_w64(v >= 0);
+  if (has != 0 && (int)(threadIdx.x & 63) == 63 - __builtin_clzll(has)) atomicMax(to, v);
+}
 
 // A row's segments in the hands of THREADS threads, `per` consecutive ones each (up to PER, kept in registers).
 template <class E, int THREADS, int SEGS>
@@ -461,19 +475,17 @@ struct Row {
   // their sum in front of it. All threads get it.
   DEVI int choose(int i0, const double (&mass)[PER], double front, double target) {
     double cum = front;
-    bool open = true;
+    int first = NO_INDEX, last = -1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (open && mass[i] > 1e-200) {  // (a segment without a kept logit may have a mass of 1024 times 2^-1000)
-        if (cum + mass[i] > target) {
-          atomicMin(&sh.first, i0 + i);
-          open = false;
-        } else {
-          atomicMax(&sh.last, i0 + i);
-        }
+      if (mass[i] > 1e-200) {  // (a segment without a kept logit may have a mass of 1024 times 2^-1000)
+        if (first == NO_INDEX && cum + mass[i] > target) first = i0 + i;
+        last = i0 + i;
       }
       cum += mass[i];
     }
+    lowest_of(first, &sh.first);
+    highest_of(last, &sh.last);
     __syncthreads();
     const int at = sh.first != NO_INDEX ? sh.first : sh.last;
     cum = front;
@@ -489,9 +501,11 @@ struct Row {
   // The settings that need no selection. False: others.
   DEVI bool simple() {
     if (s.top1) {  // the lowest index of the largest logit
+      int first = NO_INDEX;
 #pragma unroll
       for (int i = PER - 1; i >= 0; --i)
-        if (own_max[i] == top) atomicMin(&sh.first, begin + i);
+        if (own_max[i] == top) first = begin + i;
+      lowest_of(first, &sh.first);
       __syncthreads();
       if (wave == 0) {
         const int seg = sh.first;
@@ -587,15 +601,13 @@ struct Cut : Row<E, THREADS, SEGS> {
     min_last = use_k && use_p && s.min_p > 0.;
   }
 
-  // The first key from 0 to top_key for which `reached` holds, which it does from some key on (and at top_key): 64 probes
+  // The first key in [from, top_key] for which `reached` holds, which it does from some key on (and at top_key): 64 probes
   // a round.
   template <class F>
-  DEVI uint32_t first_key(F reached) const {
-    uint32_t from = 0, to = top_key;  // the answer lies in [from, to]
+  DEVI uint32_t first_key(uint32_t from, F reached) const {
+    uint32_t to = top_key;  // the answer lies in [from, to]
     while (from < to) {
-      const uint32_t step = (to - from) / 64 + 1;
-      const uint64_t probe64 = (uint64_t)from + (uint64_t)step * lane;
-      const uint32_t probe = probe64 < to ? (uint32_t)probe64 : to;
+      const uint32_t step = (to - from) / 64 + 1, probe = min(from + step * lane, to);  // (keys end far below 2^32 - 64)
       const unsigned long long hit = __builtin_amdgcn_ballot_w64(reached(probe));
       if (hit == 0) {  // behind the last probe
         from = __builtin_amdgcn_readlane(probe, 63) + 1;
@@ -658,10 +670,7 @@ struct Cut : Row<E, THREADS, SEGS> {
     }
     // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
     if (s.min_p > 0.) {
-      min_key = first_key([&](uint32_t key) {
-        const float x = value_of(key);
-        return x == x && weight_of(x, m, s.c) >= s.min_p;  // (the lowest keys are NaN's, and -inf's)
-      });
+      min_key = first_key(key_of(low), [&](uint32_t key) { return weight_of(value_of(key), m, s.c) >= s.min_p; });
       if (!min_last) low = fmaxf(low, value_of(min_key));
     }
     if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
@@ -709,23 +718,14 @@ struct Cut : Row<E, THREADS, SEGS> {
   }
 
   DEVI int base_of(int i) const { return (int)sh.active[i] * SEG; }
-  DEVI void load_active(int i, Raw<E>& x) const { load_raw<E>(x_row, base_of(i), a.V, lane, x); }
-  // f(logits, i) of active segment i, a wave each; the loads of AHEAD segments (4 KB) are under way at a time
-  static constexpr int AHEAD = VEC / 2;
+  // f(logits, i) of active segment i, a wave each (the loads of two or four segments ahead of the first's use change nothing:
+  // other waves' are under way)
   template <class F>
   DEVI void sweep(F f) {
-    for (int i0 = wave; i0 < n_active; i0 += AHEAD * WAVES) {
-      Raw<E> raw[AHEAD];
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (i0 + k * WAVES < n_active) load_active(i0 + k * WAVES, raw[k]);
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k)
-        if (i0 + k * WAVES < n_active) {
-          float x[SEG_LANE];
-          widen_raw<E>(raw[k], x);
-          f(x, i0 + k * WAVES);
-        }
+    for (int i = wave; i < n_active; i += WAVES) {
+      float x[SEG_LANE];
+      load_seg<E>(x_row, base_of(i), a.V, lane, x);
+      f(x, i);
     }
   }
   // Appends the logits marked by `flags` (bit j: element j of the lane) to a list, in index order from entry `to` on.
@@ -888,7 +888,8 @@ struct Cut : Row<E, THREADS, SEGS> {
   }
   // (cut_index is read behind a barrier)
   DEVI double kept_weight(float x, uint32_t key, int at) const {
-    return key > cut_key || (key == cut_key && at <= sh.cut_index) ? weight_of(x, m, s.c) : 0.;
+    const double e = weight_of(x, m, s.c);  // (in front of the choice: no branch per element)
+    return key > cut_key || (key == cut_key && at <= sh.cut_index) ? e : 0.;
   }
   // The list's part of the kept set: weights in place of keys, each segment's into its mass (ADD: added). Sixteen lanes
   // per segment.
@@ -1013,19 +1014,19 @@ struct Cut : Row<E, THREADS, SEGS> {
     const unsigned long long low_mass = (unsigned long long)fmax(ceil(least - off), 0.);
     const unsigned long long high_mass = (unsigned long long)ceil(least + off);
     unsigned long long front = 0;
-    int first_low = BINS, first_high = BINS;
+    int first_low = NO_INDEX, first_high = NO_INDEX;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
       const unsigned long long next = cum + h[i];
-      if (first_low == BINS && next >= low_mass) {
+      if (first_low == NO_INDEX && next >= low_mass) {
         first_low = tid * OWN + i;
         front = cum;
       }
-      if (first_high == BINS && next >= high_mass) first_high = tid * OWN + i;
+      if (first_high == NO_INDEX && next >= high_mass) first_high = tid * OWN + i;
       cum = next;
     }
-    if (first_low < BINS) atomicMin(&sh.bin_low, first_low);
-    if (first_high < BINS) atomicMin(&sh.bin_high, first_high);
+    lowest_of(first_low, &sh.bin_low);
+    lowest_of(first_high, &sh.bin_high);
     __syncthreads();
     if (first_low == sh.bin_low) sh.above = front;  // (a count, for top-k)
     want = NO_INDEX;
@@ -1036,9 +1037,8 @@ struct Cut : Row<E, THREADS, SEGS> {
     // the bins' limits as logits: the lowest of bins up to one
     if (wave < 2) {
       const int bin = wave == 0 ? sh.bin_low - 1 : sh.bin_high;
-      const float limit = bin < 0 ? pos_inf() : value_of(first_key([&](uint32_t key) {
-        const float x = value_of(key);
-        return x >= low && bin_of(depth_of(x)) <= bin;
+      const float limit = bin < 0 ? pos_inf() : value_of(first_key(key_of(low), [&](uint32_t key) {
+        return bin_of(depth_of(value_of(key))) <= bin;
       }));
       if (lane == 0) sh.limits[wave] = limit;
     }
@@ -1098,9 +1098,7 @@ struct Cut : Row<E, THREADS, SEGS> {
     if (wave == 0 && sh.bin >= 0) {
       const int i = sh.bin;
       float x[SEG_LANE];
-      Raw<E> raw;
-      load_active(i, raw);
-      widen_raw<E>(raw, x);
+      load_seg<E>(x_row, base_of(i), a.V, lane, x);
       unsigned flags = 0;
 #pragma unroll
       for (int j = 0; j < SEG_LANE; ++j) flags |= (x[j] >= low && key_of(x[j]) == cut_key ? 1u : 0u) << j;
@@ -1132,12 +1130,12 @@ struct Cut : Row<E, THREADS, SEGS> {
       const int base = base_of(chosen);
       float x[SEG_LANE];
       double w[SEG_LANE];
-      Raw<E> raw;
-      load_active(chosen, raw);
-      widen_raw<E>(raw, x);
+      load_seg<E>(x_row, base, a.V, lane, x);
 #pragma unroll
-      for (int j = 0; j < SEG_LANE; ++j)
-        w[j] = x[j] >= low ? kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane)) : 0.;
+      for (int j = 0; j < SEG_LANE; ++j) {
+        const double e = kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane));
+        w[j] = x[j] >= low ? e : 0.;
+      }
       const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
       finish_cut(token, z);
     }
@@ -1382,7 +1380,7 @@ struct Layout {
     sub_max = take(rows * segs * SUBS * 4);
     cut = take(rows * 4);
     cut_index = take(rows * 4);
-    parts = segs <= FEW_SEGS && n <= SPREAD_ROWS ? ceil_div_i64(segs, PART) : 0;
+    parts = segs >= SPREAD_SEGS && segs <= FEW_SEGS && n <= SPREAD_ROWS ? ceil_div_i64(segs, PART) : 0;
     spread = take(parts ? rows * (int64_t)sizeof(Spread) : 0);
     part_bins = take(rows * parts * BINS * 8);
     part_mass = take(parts ? rows * segs * 8 : 0);

@@ -198,7 +198,7 @@ int areal_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t N, in
  * whose bit is set in kept (as above; other logits are not looked at, whatever they hold). A label in
  * [0, V) that is not kept, or whose logit is -inf: -inf. A row that keeps nothing above -inf: -inf
  * and entropy 0. A label outside [0, V): 0. A kept NaN or +inf: NaN. lse2 (NULL to skip): what
- * the backward needs besides the entropy. */
+ * the backward needs besides the entropy. N is at most 2^22, V 2^30, else AREAL_ERR_UNSUPPORTED. */
 int areal_kept_logprobs_entropy_fwd(const void* logits, int dtype, int64_t ld,
                                     const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
                                     int64_t N, int64_t V, float inv_temperature, float* logprobs,
