@@ -937,13 +937,13 @@ struct KeptLogits : public torch::autograd::Function<KeptLogits> {
     const Tensor lab = flat(labels, at::kLong);
     const Tensor words = kept.reshape({N, kept.size(-1)}).contiguous();
     const Tensor lp = empty(rows, labels.sizes(), at::kFloat), ent = empty(rows, labels.sizes(), at::kFloat);
-    const Tensor lse2 = needs_grad ? empty_f32(rows, N) : Tensor();
+    const Tensor stats = needs_grad ? empty_f32(rows, 2 * N) : Tensor();
     check(areal_kept_logprobs_entropy_fwd(ptr<void>(rows), dtype_code(rows.scalar_type()), pitch_of(rows),
                                           ptr<int64_t>(lab), ptr<uint32_t>(words), words.size(1), N, V,
                                           (float)(1.0 / temperature), ptr<float>(lp), ptr<float>(ent),
-                                          ptr<float>(lse2), stream_of(rows)),
+                                          ptr<float>(stats), stream_of(rows)),
           "areal_kept_logprobs_entropy_fwd");
-    ctx->save_for_backward({rows, lab, words, lse2, ent});
+    ctx->save_for_backward({rows, lab, words, stats, ent});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["shape"] = logits.sizes().vec();
     ctx->saved_data["type"] = (int64_t)logits.scalar_type();
@@ -954,14 +954,14 @@ struct KeptLogits : public torch::autograd::Function<KeptLogits> {
     variable_list r(5);
     if (!grads[0].defined() && !grads[1].defined()) return r;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &rows = saved[0], &lab = saved[1], &words = saved[2], &lse2 = saved[3], &ent = saved[4];
+    const Tensor &rows = saved[0], &lab = saved[1], &words = saved[2], &stats = saved[3], &ent = saved[4];
     const c10::hip::HIPGuard guard(rows.device().index());
     const int64_t N = rows.size(0), V = rows.size(1);
     const Tensor glp = flat(grads[0], at::kFloat), gen = flat(grads[1], at::kFloat);
     Tensor d = empty(rows, {N, V}, rows.scalar_type());
     check(areal_kept_logprobs_entropy_bwd(ptr<void>(rows), dtype_code(rows.scalar_type()), pitch_of(rows),
                                           ptr<int64_t>(lab), ptr<uint32_t>(words), words.size(1), N, V,
-                                          (float)(1.0 / ctx->saved_data["temperature"].toDouble()), ptr<float>(lse2),
+                                          (float)(1.0 / ctx->saved_data["temperature"].toDouble()), ptr<float>(stats),
                                           ptr<float>(ent), ptr<float>(glp), ptr<float>(gen), ptr<void>(d), V,
                                           stream_of(rows)),
           "areal_kept_logprobs_entropy_bwd");

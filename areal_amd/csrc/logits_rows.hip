@@ -348,6 +348,8 @@ int launch_rows_bwd(const void* logits, int64_t ld, const int64_t* labels, int64
 // Bit j of word w of a row stands for token 32 w + j. A wave takes 2048 tokens at a time: a word per lane, and where
 // one is not empty each lane the logits of four of their bytes, 512 tokens in one step. Logits without a bit are not
 // looked at (8 neighbours without one not even read), so a row that keeps few costs its bits.
+// Maxima are logits, and exponents (x - max) * c2: the lowest value of a type times c2 would be -inf, which a row that keeps
+// nothing else must not be.
 constexpr int64_t KEPT_MAX_ROWS = BWD_MAX_BLOCKS / 2;  // a block of up to 1024 threads each
 constexpr int KEPT_STEP = 2048, KEPT_UNIT = 8, KEPT_STEPS = 4;
 // Exponents are held above this: a kept logit of -inf then adds 0 to sums of t * 2^t (a NaN stays one).
@@ -400,9 +402,41 @@ DEVI void load_kept_end(const T* x, int c, int V, uint32_t word, int lane, uint3
 }
 DEVI bool kept_at(const uint32_t* kept, int64_t token) { return kept[token >> 5] >> (token & 31) & 1; }
 
+// As Online, with the largest logit itself for m.
+struct KeptOnline {
+  float m, s, q;
+};
+DEVI void kept_merge(KeptOnline& a, const KeptOnline& b, float c2) {
+  const float m = fmaxf(a.m, b.m);
+  float s = 0.f, q = 0.f;
+  auto part = [&](const KeptOnline& o) {
+    const float d = o.m > neg_inf() ? stat_max((o.m - m) * c2, KEPT_LOWEST) : 0.f, al = fast_exp2(d);
+    s += al * o.s;
+    q += al * fmaf(d, o.s, o.q);
+  };
+  part(a);
+  part(b);
+  a.m = m; a.s = s; a.q = q;
+}
+// Of a workgroup of WAVES.
+template <int WAVES>
+DEVI KeptOnline kept_merge_block(KeptOnline st, KeptOnline* smem, float c2) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const KeptOnline other{__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.q, o, 64)};
+    kept_merge(st, other, c2);
+  }
+  if ((threadIdx.x & 63) == 0) smem[threadIdx.x >> 6] = st;
+  __syncthreads();
+  KeptOnline r = smem[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) kept_merge(r, smem[i], c2);
+  return r;
+}
+
 // Adds the logits of a lane's units whose bits are set. ALL: all are.
 template <bool ALL>
-DEVI void online_add_kept(Online& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], float c2) {
+DEVI void online_add_kept(KeptOnline& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], float c2) {
   float xm = neg_inf();
 #pragma unroll
   for (int k = 0; k < KEPT_STEPS; ++k)
@@ -411,14 +445,13 @@ DEVI void online_add_kept(Online& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const u
       if (!ALL) z[k][i] = b[k] >> i & 1 ? z[k][i] : neg_inf();
       xm = fmaxf(xm, z[k][i]);
     }
-  const float vm = xm * c2;
-  if (vm > st.m) {
+  if (xm > st.m) {
     if (st.m > neg_inf()) {
-      const float d = st.m - vm, al = fast_exp2(d);
+      const float d = stat_max((st.m - xm) * c2, KEPT_LOWEST), al = fast_exp2(d);
       st.q = al * fmaf(d, st.s, st.q);
       st.s = al * st.s;
     }
-    st.m = vm;
+    st.m = xm;
   }
   const float m = st.m > neg_inf() ? st.m : 0.f;
 #pragma unroll
@@ -426,7 +459,7 @@ DEVI void online_add_kept(Online& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const u
     if (!ALL && __builtin_amdgcn_ballot_w64(b[k] != 0) == 0) continue;
 #pragma unroll
     for (int i = 0; i < KEPT_UNIT; ++i) {
-      const float t = stat_max(fmaf(z[k][i], c2, -m), KEPT_LOWEST);
+      const float t = stat_max((z[k][i] - m) * c2, KEPT_LOWEST);
       const float e = fast_exp2(t);
       st.s += e;
       st.q = fmaf(t, e, st.q);
@@ -442,15 +475,15 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
                                                            const int64_t* __restrict__ labels,
                                                            const uint32_t* __restrict__ kept, int64_t kept_ld, int V,
                                                            float inv_temp, float* __restrict__ logprobs,
-                                                           float* __restrict__ entropy, float* __restrict__ lse2_out) {
-  __shared__ Online smem[THREADS / 64];
+                                                           float* __restrict__ entropy, float2* __restrict__ stats) {
   constexpr int WAVES = THREADS / 64, AHEAD = 4;
+  __shared__ KeptOnline smem[WAVES];
   const int64_t row = blockIdx.x;
   const T* const x = logits + row * ld;
   const uint32_t* const bits = kept + row * kept_ld;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float c2 = inv_temp * LOG2E_F;
-  Online st{neg_inf(), 0.f, 0.f};
+  KeptOnline st{neg_inf(), 0.f, 0.f};
   auto add = [&](float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], uint32_t word) {
     if (__builtin_amdgcn_ballot_w64(word == 0xffffffffu) == ~0ull) online_add_kept<true>(st, z, b, c2);
     else if (__builtin_amdgcn_ballot_w64(word != 0) != 0) online_add_kept<false>(st, z, b, c2);
@@ -483,7 +516,7 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
     load_kept_end<T>(x, c, V, word, lane, b, z);
     add(z, b, word);
   }
-  const Online r = block_merge(st, smem);
+  const KeptOnline r = kept_merge_block<WAVES>(st, smem, c2);
   if (threadIdx.x == 0) {
     const float log2s = fast_log2(r.s);
     const bool none = r.m == neg_inf() && r.s == 0.f;  // no kept logit above -inf
@@ -494,13 +527,13 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
     } else if (lab >= 0 && lab < V) {
       lp = neg_inf();
       if (!none && kept_at(bits, lab)) {
-        lp = (fmaf(Elem<T>::load(x + lab), c2, -r.m) - log2s) * LN2_F;
+        lp = fmaf(Elem<T>::load(x + lab) - r.m, inv_temp, -log2s * LN2_F);
         lp = lp > 0.f ? 0.f : lp;
       }
     }
     logprobs[row] = lp;
     if (entropy) entropy[row] = none ? 0.f : (log2s - r.q / r.s) * LN2_F;
-    if (lse2_out) lse2_out[row] = none ? pos_inf() : r.m + log2s;  // +inf: every probability is 0
+    if (stats) stats[row] = none ? make_float2(0.f, pos_inf()) : make_float2(r.m, log2s);  // +inf: every probability is 0
   }
 }
 
@@ -510,7 +543,7 @@ constexpr int KEPT_BWD_WAVES = 4;
 template <typename T, bool ENT>
 __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
     const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ labels, const uint32_t* __restrict__ kept,
-    int64_t kept_ld, int V, float inv_temp, const float* __restrict__ lse2, const float* __restrict__ entropy,
+    int64_t kept_ld, int V, float inv_temp, const float2* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ grad_lp, const float* __restrict__ grad_ent, T* __restrict__ dlogits, int64_t ldd,
     unsigned parts, unsigned part_steps) {
   constexpr int VEC = Elem<T>::VEC;
@@ -521,7 +554,7 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
   const uint32_t* const bits = kept + row * kept_ld;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float c2 = inv_temp * LOG2E_F;
-  const float l2 = lse2[row];
+  const float m = stats[row].x, log2s = stats[row].y;
   const int64_t lab64 = labels[row];
   // a label outside the kept set has log-probability -inf, whose gradient is taken as 0
   const bool labelled = lab64 >= 0 && lab64 < V && kept_at(bits, lab64) && !(Elem<T>::load(x + lab64) == neg_inf());
@@ -529,7 +562,7 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
   const float glp = labelled && grad_lp ? grad_lp[row] * inv_temp : 0.f;
   const float gen = ENT ? grad_ent[row] * inv_temp : 0.f;
   const float ent = ENT ? entropy[row] : 0.f;
-  const bool none = l2 == pos_inf();
+  const bool none = log2s == pos_inf();
   for (unsigned step = wave; step < part_steps; step += KEPT_BWD_WAVES) {
     const int64_t c64 = ((int64_t)part * part_steps + step) * KEPT_STEP;
     if (c64 >= V) return;
@@ -567,7 +600,7 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
       if (b[i] != 0) {
 #pragma unroll
         for (int j = 0; j < KEPT_UNIT; ++j) {
-          const float t = stat_max(fmaf(z[i][j], c2, -l2), KEPT_LOWEST);
+          const float t = stat_max(fmaf(z[i][j] - m, c2, -log2s), KEPT_LOWEST);
           const float p = fast_exp2(t);
           float v = -p * glp;
           if (at + j == lab) v += glp;
@@ -587,13 +620,17 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
   }
 }
 
+// The factor of the exponents is finite, and the difference of two logits is out of fp32's range only where the product would
+// be far below 0 too.
+bool kept_temperature(float inv_temperature) { return inv_temperature > 0.9e-30f && inv_temperature < 2e38f; }
+
 template <typename T>
 int launch_kept_fwd(const void* logits, int64_t ld, const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
-                    int64_t N, int64_t V, float inv_temp, float* lp, float* ent, float* lse2, hipStream_t stream) {
+                    int64_t N, int64_t V, float inv_temp, float* lp, float* ent, float* stats, hipStream_t stream) {
   auto launch = [&](auto threads) {
     constexpr int THREADS = decltype(threads)::value;
     hipLaunchKernelGGL((kept_fwd_kernel<T, THREADS>), dim3((unsigned)N), dim3(THREADS), 0, stream, (const T*)logits, ld,
-                       labels, kept, kept_ld, (int)V, inv_temp, lp, ent, lse2);
+                       labels, kept, kept_ld, (int)V, inv_temp, lp, ent, (float2*)stats);
   };
   if (N < FWD_FEW_ROWS)
     launch(std::integral_constant<int, 512>{});
@@ -605,7 +642,7 @@ int launch_kept_fwd(const void* logits, int64_t ld, const int64_t* labels, const
 
 template <typename T>
 int launch_kept_bwd(const void* logits, int64_t ld, const int64_t* labels, const uint32_t* kept, int64_t kept_ld,
-                    int64_t N, int64_t V, float inv_temp, const float* lse2, const float* ent, const float* glp,
+                    int64_t N, int64_t V, float inv_temp, const float* stats, const float* ent, const float* glp,
                     const float* gent, void* dlogits, int64_t ldd, hipStream_t stream) {
   const int64_t steps = ceil_div_i64(V, KEPT_STEP);
   int64_t parts = ceil_div_i64(steps, KEPT_BWD_WAVES);
@@ -614,7 +651,7 @@ int launch_kept_bwd(const void* logits, int64_t ld, const int64_t* labels, const
   auto launch = [&](auto with_entropy) {
     hipLaunchKernelGGL((kept_bwd_kernel<T, decltype(with_entropy)::value>), dim3((unsigned)(N * parts)),
                        dim3(64 * KEPT_BWD_WAVES), 0, stream, (const T*)logits, ld, labels, kept, kept_ld, (int)V,
-                       inv_temp, lse2, ent, glp, gent, (T*)dlogits, ldd, (unsigned)parts, (unsigned)part_steps);
+                       inv_temp, (const float2*)stats, ent, glp, gent, (T*)dlogits, ldd, (unsigned)parts, (unsigned)part_steps);
   };
   if (gent)
     launch(std::true_type{});
@@ -673,30 +710,32 @@ int areal_logits_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld,
 // dtype: 0 = fp32, 1 = bf16, 2 = fp16. kept [N, kept_ld] words.
 int areal_kept_logprobs_entropy_fwd(const void* logits, int dtype, int64_t ld, const int64_t* labels,
                                     const uint32_t* kept, int64_t kept_ld, int64_t N, int64_t V, float inv_temperature,
-                                    float* logprobs, float* entropy, float* lse2, hipStream_t stream) {
-  if (N < 0 || V <= 0 || ld < V || kept_ld < ceil_div_i64(V, 32) || !(inv_temperature > 0.f)) return AREAL_ERR_BAD_ARG;
+                                    float* logprobs, float* entropy, float* stats, hipStream_t stream) {
+  if (N < 0 || V <= 0 || ld < V || kept_ld < ceil_div_i64(V, 32) || !kept_temperature(inv_temperature)) return AREAL_ERR_BAD_ARG;
   if (N == 0) return AREAL_OK;
   if (!logits || !labels || !kept || !logprobs) return AREAL_ERR_BAD_ARG;
   if (V > (1 << 30) || N > KEPT_MAX_ROWS) return AREAL_ERR_UNSUPPORTED;
+  if (!aligned_to(stats, 8)) return AREAL_ERR_ALIGNMENT;
   auto run = [&](auto t) {
     return launch_kept_fwd<decltype(t)>(logits, ld, labels, kept, kept_ld, N, V, inv_temperature, logprobs, entropy,
-                                        lse2, stream);
+                                        stats, stream);
   };
   return dtype == 0 ? run(float{}) : dtype == 1 ? run(u16{}) : dtype == 2 ? run(_Float16{}) : AREAL_ERR_BAD_ARG;
 }
 
 int areal_kept_logprobs_entropy_bwd(const void* logits, int dtype, int64_t ld, const int64_t* labels,
                                     const uint32_t* kept, int64_t kept_ld, int64_t N, int64_t V, float inv_temperature,
-                                    const float* lse2, const float* entropy, const float* grad_logprobs,
+                                    const float* stats, const float* entropy, const float* grad_logprobs,
                                     const float* grad_entropy, void* dlogits, int64_t ldd, hipStream_t stream) {
-  if (N < 0 || V <= 0 || ld < V || ldd < V || kept_ld < ceil_div_i64(V, 32) || !(inv_temperature > 0.f))
+  if (N < 0 || V <= 0 || ld < V || ldd < V || kept_ld < ceil_div_i64(V, 32) || !kept_temperature(inv_temperature))
     return AREAL_ERR_BAD_ARG;
   if (N == 0) return AREAL_OK;
-  if (!logits || !labels || !kept || !lse2 || !dlogits) return AREAL_ERR_BAD_ARG;
+  if (!logits || !labels || !kept || !stats || !dlogits) return AREAL_ERR_BAD_ARG;
   if (grad_entropy != nullptr && entropy == nullptr) return AREAL_ERR_BAD_ARG;
   if (V > (1 << 30) || N > KEPT_MAX_ROWS) return AREAL_ERR_UNSUPPORTED;
+  if (!aligned_to(stats, 8)) return AREAL_ERR_ALIGNMENT;
   auto run = [&](auto t) {
-    return launch_kept_bwd<decltype(t)>(logits, ld, labels, kept, kept_ld, N, V, inv_temperature, lse2, entropy,
+    return launch_kept_bwd<decltype(t)>(logits, ld, labels, kept, kept_ld, N, V, inv_temperature, stats, entropy,
                                         grad_logprobs, grad_entropy, dlogits, ldd, stream);
   };
   return dtype == 0 ? run(float{}) : dtype == 1 ? run(u16{}) : dtype == 2 ? run(_Float16{}) : AREAL_ERR_BAD_ARG;

@@ -126,7 +126,7 @@ def gather_kept_logprobs_entropy(
             that are not kept does not matter, NaN and infinities included.
         labels: ``[...]`` integer labels.
         kept: int32 ``[..., W]``, ``W >= ceil(V / 32)``, as ``sample_tokens`` returns it; words of -1 keep all.
-        temperature: softmax temperature (> 0).
+        temperature: softmax temperature, in [1e-38, 1e30].
 
     A label that is not kept has log-probability ``-inf``, without a gradient (leave such tokens out
     of the loss); a row that keeps nothing has entropy 0 as well. A label outside ``[0, V)`` (an ignored
@@ -134,6 +134,8 @@ def gather_kept_logprobs_entropy(
     """
     if not math.isfinite(temperature) or temperature <= 0:
         raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 1e-38 <= temperature <= 1e30:
+        raise ValueError(f"temperature must lie in [1e-38, 1e30], got {temperature}")
     if logits.ndim == 0 or logits.size(-1) == 0:
         raise ValueError(f"logits must have at least one element per row, got {tuple(logits.shape)}")
     if not logits.is_floating_point():

@@ -111,6 +111,73 @@ def test_kept_values_that_are_not_finite(dev, dtype):
     assert lp[3] == lp[4] == -math.inf and ent[4] == 0
 
 
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.5, 1e-38, 1e30])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_keep_only_lowest_values(dev, dtype, tau):
+    """Masking with the type's lowest finite value: a row that keeps nothing else is uniform, not empty."""
+    g = torch.Generator().manual_seed(7)
+    n, v = 6, 4500
+    low, top = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.full((n, v), low, dtype=dtype)
+    mask = torch.rand(n, v, generator=g) < 0.3
+    mask[0] = True
+    labels = torch.tensor([int(torch.nonzero(m)[9]) for m in mask])
+    x[1, ~mask[1]] = top                 # not kept
+    x[2, labels[2]] = top                # all of the mass (or, in fp16 at the highest temperature, its share)
+    alone = (top - low) / tau > 1e3
+    x[3, torch.nonzero(mask[3])[50:, 0]] = -math.inf
+    x[4, labels[4]] = -math.inf
+    mask[5], labels[5] = False, 4499
+    mask[5, 4499] = True                 # one, at the end
+    count = torch.tensor([v, int(mask[1].sum()), 1 if alone else int(mask[2].sum()), 50, int(mask[4].sum()) - 1, 1]).double()
+    glp, gent = torch.randn(n, generator=g), torch.randn(n, generator=g)
+    xg = x.to(dev).requires_grad_(True)
+    lp, ent = gather_kept_logprobs_entropy(xg, labels.to(dev), O.pack_bits(mask).to(dev), tau)
+    # exponents are 0 or below the lowest: one rounding each of the logarithm (2 units), its product and ln 2
+    want = -count.log()
+    want[4] = -math.inf
+    torch.testing.assert_close(lp.detach().cpu().double(), want, rtol=2.0**-21, atol=0)
+    torch.testing.assert_close(ent.detach().cpu().double(), count.log(), rtol=2.0**-21, atol=0)
+    # p is off by the exponent's rounding (log2 of the count, 13 at most, in 2 units) and the exponential's
+    (d,) = torch.autograd.grad(lp, xg, glp.to(dev), retain_graph=True)
+    p = (mask & (x > -math.inf)).double() / count[:, None]
+    if alone:
+        p[2] = 0.0
+        p[2, labels[2]] = 1.0
+    one = torch.zeros(n, v, dtype=torch.float64).scatter_(1, labels[:, None], 1.0)
+    want = glp.double()[:, None] * (one - p) / tau
+    want[4] = 0.0
+    cap = torch.finfo(dtype).max
+    scale = glp.double().abs()[:, None] / tau
+    bound = scale * p * 2.0**-18 + scale * one * 2.0**-22 + torch.finfo(dtype).eps / 2 * want.abs()
+    bound = bound + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    fits = want.abs() < cap
+    off = (d.cpu().double() - want).abs()
+    assert (off[fits] <= bound[fits]).all(), (off[fits] - bound[fits]).max()
+    # p (log p + entropy) is 0 in a uniform row, up to the errors of both logarithms
+    (d,) = torch.autograd.grad(ent, xg, gent.to(dev))
+    bound = gent.double().abs()[:, None] / tau * p * (2.0**-18 * (1 + count.log()[:, None]))
+    bound = bound + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    # (times 1 / tau = 1e38 the errors alone, 2^-24 and up, are 6e30: out of fp16's range they are rounded to infinity)
+    bound = torch.where(bound > cap, math.inf, bound)
+    assert (d.cpu().double().abs() <= bound).all()
+
+
+def test_a_label_of_the_lowest_value(dev):
+    x = torch.zeros(2, 40, device=dev)
+    x[:, 7] = torch.finfo(torch.float32).min
+    x[1, 3] = torch.finfo(torch.float32).max
+    xg = x.requires_grad_(True)
+    words = torch.full((2, 2), -1, dtype=torch.int32, device=dev)
+    lp, ent = gather_kept_logprobs_entropy(xg, torch.tensor([7, 7], device=dev), words)
+    assert lp[0] == torch.finfo(torch.float32).min and lp[1] == -math.inf  # -6.8e38 is out of range
+    torch.testing.assert_close(ent.detach().cpu(), torch.tensor([math.log(39), 0.0]), rtol=2.0**-21, atol=0)
+    (d,) = torch.autograd.grad(lp, xg, torch.ones(2, device=dev))
+    torch.testing.assert_close(d[0].cpu(), torch.full((40,), -1 / 39).index_fill_(0, torch.tensor(7), 1.0),
+                               rtol=2.0**-18, atol=0)
+    assert torch.isfinite(d).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layouts(dev, dtype):
     """Rows of any start and pitch, more words than the vocabulary needs and bits behind it, more dimensions."""

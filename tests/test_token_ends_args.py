@@ -39,6 +39,8 @@ W, I = torch.zeros(6, 8), torch.zeros(4, dtype=torch.long)
     (lambda: sample_tokens(X, U, min_p=torch.zeros(3, 1)), "min_p must have one value per row"),
     (lambda: gather_kept_logprobs_entropy(X, Y, K, 0.0), "temperature must be positive"),
     (lambda: gather_kept_logprobs_entropy(X, Y, K, math.nan), "temperature must be positive"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K, 1e-39), "temperature must lie"),
+    (lambda: gather_kept_logprobs_entropy(X, Y, K, 1e31), "temperature must lie"),
     (lambda: gather_kept_logprobs_entropy(X, Y[:2], K), "must match labels"),
     (lambda: gather_kept_logprobs_entropy(X, Y, K.long()), "kept must be int32"),
     (lambda: gather_kept_logprobs_entropy(X, Y, K[:, :1]), "2 words for each label"),
@@ -111,6 +113,9 @@ def test_c_entries_refuse_before_a_launch():
 
     assert kept(N=0) == 0
     assert kept(ld=39) == kept(words=1) == kept(inv=0.0) == kept(inv=math.nan) == kept(k=null) == kept(lab=null) == bad
+    assert kept(inv=math.inf) == kept(inv=2.1e38) == kept(inv=1e-31) == bad
+    odd = ctypes.c_void_p(4100)
+    assert lib.areal_kept_logprobs_entropy_fwd(p, 1, 40, p, p, 2, 3, 40, 1.0, p, p, odd, null) == -2
     assert kept(dtype=3) == kept(N=-1) == kept(V=0) == bad and kept(V=(1 << 30) + 1, ld=1 << 31, words=1 << 26) == unsupported
     assert lib.areal_kept_logprobs_entropy_bwd(p, 1, 40, p, p, 2, 3, 40, 1.0, p, null, p, p, p, 40, null) == bad
 
