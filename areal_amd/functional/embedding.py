@@ -5,8 +5,6 @@
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from areal_amd import _lib
@@ -49,8 +47,8 @@ def embed_tokens(
         raise ValueError(f"out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
     if input_ids.is_floating_point() or input_ids.is_complex() or input_ids.dtype == torch.bool:
         raise ValueError(f"input_ids must be integers, got {input_ids.dtype}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale must be finite in fp32, got {scale}")
     if padding_idx is not None and not 0 <= padding_idx < weight.size(0):
         raise ValueError(f"padding_idx must lie in [0, {weight.size(0)}), got {padding_idx}")
     if weight_grad_accum is not None:

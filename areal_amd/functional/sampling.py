@@ -72,8 +72,9 @@ def sample_tokens(
         logits: ``[..., V]``, fp32, bf16 or fp16 (other types are converted to fp32), ``V`` up to
             ``MAX_VOCAB``; logits of ``-inf`` are never drawn.
         uniforms: ``[...]`` fp32 or fp64 numbers in ``[0, 1)`` (others are clamped, a NaN counts as 0).
-        temperature: a number >= 0, or a tensor with one per row; 0 (or below, in a tensor) takes the
-            first of the largest logits, with log-probabilities 0.
+        temperature: a number >= 0, or a tensor with one per row (taken in fp32, as those of top_p and min_p;
+            numbers are taken in fp64); 0 (or below, in a tensor) takes the first of the largest logits, with
+            log-probabilities 0.
         top_k: a number, or an integer tensor; ``None``, 0 and below: no limit.
         top_p: a number in (0, 1], or a tensor (1 and above: no limit, 0 and below: the first alone).
         min_p: a number in [0, 1], or a tensor (clamped to that).

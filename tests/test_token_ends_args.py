@@ -54,6 +54,8 @@ W, I = torch.zeros(6, 8), torch.zeros(4, dtype=torch.long)
     (lambda: embed_tokens(I.float(), W), "input_ids must be integers"),
     (lambda: embed_tokens(I > 0, W), "input_ids must be integers"),
     (lambda: embed_tokens(I, W, math.inf), "scale must be finite"),
+    (lambda: embed_tokens(I, W, 1e39), "scale must be finite"),
+    (lambda: embed_tokens(I, W, math.nan), "scale must be finite"),
     (lambda: embed_tokens(I, W, padding_idx=6), "padding_idx must lie"),
     (lambda: embed_tokens(I, W, padding_idx=-1), "padding_idx must lie"),
     (lambda: embed_tokens(I, W, weight_grad_accum=W.bfloat16()), "weight_grad_accum must be an fp32"),
