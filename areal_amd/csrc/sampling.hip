@@ -720,13 +720,17 @@ struct Cut : Row<E, THREADS, SEGS> {
   DEVI int base_of(int i) const { return (int)sh.active[i] * SEG; }
   // f(logits, i) of active segment i, a wave each (the loads of two or four segments ahead of the first's use change nothing:
   // other waves' are under way)
-  template <class F>
-  DEVI void sweep(F f) {
-    for (int i = wave; i < n_active; i += WAVES) {
+  template <class F, class Done>
+  DEVI void sweep_until(Done done, F f) {
+    for (int i = wave; i < n_active && !done(); i += WAVES) {
       float x[SEG_LANE];
       load_seg<E>(x_row, base_of(i), a.V, lane, x);
       f(x, i);
     }
+  }
+  template <class F>
+  DEVI void sweep(F f) {
+    sweep_until([] { return false; }, f);
   }
   // Appends the logits marked by `flags` (bit j: element j of the lane) to a list, in index order from entry `to` on.
   DEVI void append(const float (&x)[SEG_LANE], unsigned flags, int (&starts)[G], int to, int base, uint2* entry,
@@ -744,11 +748,11 @@ struct Cut : Row<E, THREADS, SEGS> {
     }
   }
   // The logits that flags_of(logits, i) marks, as the list; segments take runs of it in any order. Once they are too many
-  // for it, segments are left out.
+  // for it, the other segments are not read (512 x 128256 bf16 with top-p 0.9: 13 us less).
   template <class F>
   DEVI void collect(F flags_of) {
-    sweep([&](const float (&x)[SEG_LANE], int i) {
-      if (*(volatile int*)&sh.n_list > LIST) return;
+    auto full = [&] { return __builtin_amdgcn_readfirstlane(*(volatile int*)&sh.n_list) > LIST; };
+    sweep_until(full, [&](const float (&x)[SEG_LANE], int i) {
       const unsigned flags = flags_of(x, i);
       int starts[G];
       const int own = order_in_wave<E>(flags, starts);
@@ -891,8 +895,9 @@ struct Cut : Row<E, THREADS, SEGS> {
     const double e = weight_of(x, m, s.c);  // (in front of the choice: no branch per element)
     return key > cut_key || (key == cut_key && at <= sh.cut_index) ? e : 0.;
   }
-  // The list's part of the kept set: weights in place of keys, each segment's into its mass (ADD: added). Sixteen lanes
-  // per segment.
+  // The list's part of the kept set: weights in place of keys, each segment's into its mass (ADD: added). An entry per
+  // thread first (as a segment's may be a hundred), then sixteen lanes per segment add: 77 x 32000 with top-p
+  // 0.9 9,400 clocks, with both by sixteen lanes 11,800.
   template <bool ADD>
   DEVI void weigh_list() {
     if (take != NO_INDEX) {
@@ -916,15 +921,14 @@ struct Cut : Row<E, THREADS, SEGS> {
       }
       __syncthreads();
     }
+    for (int j = tid; j < n_list; j += THREADS) {
+      const uint32_t key = sh.entry[j].x;
+      sh.entry[j] = __builtin_bit_cast(uint2, kept_weight(value_of(key), key, sh.index[j]));
+    }
+    __syncthreads();
     for (int i = tid / 16; i < n_active; i += THREADS / 16) {
       double w = 0.;
-      for (int j = tid % 16; j < sh.seg_count[i]; j += 16) {
-        const int at = sh.seg_first[i] + j;
-        const uint32_t key = sh.entry[at].x;
-        const double e = kept_weight(value_of(key), key, sh.index[at]);
-        sh.entry[at] = __builtin_bit_cast(uint2, e);
-        w += e;
-      }
+      for (int j = tid % 16; j < sh.seg_count[i]; j += 16) w += __builtin_bit_cast(double, sh.entry[sh.seg_first[i] + j]);
       w = row_reduce(w, [](double x, double y) { return x + y; });
       if (tid % 16 == 0) sh.seg_mass[i] = ADD ? sh.seg_mass[i] + w : w;
     }
