@@ -558,6 +558,8 @@ struct CutShared {
   unsigned long long above;
   int bin, ties, bin_low, bin_high, cut_index, n_list;
   float limits[2];
+  uint32_t min_key;
+  unsigned long long bin_mass;
   unsigned short active[SEGS];  // segments that reach the lower bound
   int seg_first[SEGS], seg_count[SEGS];  // their entries of the list: a run of it each, in index order
   int seg_ties[SEGS];
@@ -662,16 +664,28 @@ struct Cut : Row<E, THREADS, SEGS> {
     clear_bins();
     top_key = key_of(top);
     low = -3.402823466e38f;
-    if (use_p && !use_k) {
-      // No token lighter than this is in S2: all those together weigh less than (1 - top_p) of the mass.
-      double b = m + log2((1. - s.top_p) * all_mass / a.V) / s.c;
-      b -= 1e-6 * fabs(b) + 1e-6 / s.c;
-      if (b > -3.4e38) low = (float)b;
+    // One wave looks for the limits of top-p and min-p (all sixteen in turn take 2,000 clocks more).
+    if (wave == 0 && (s.min_p > 0. || (use_p && !use_k))) {
+      if (use_p && !use_k) {
+        // No token lighter than this is in S2: all those together weigh less than (1 - top_p) of the mass.
+        double b = m + log2((1. - s.top_p) * all_mass / a.V) / s.c;
+        b -= 1e-6 * fabs(b) + 1e-6 / s.c;
+        if (b > -3.4e38) low = (float)b;
+      }
+      // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
+      if (s.min_p > 0.) {
+        min_key = first_key(key_of(low), [&](uint32_t key) { return weight_of(value_of(key), m, s.c) >= s.min_p; });
+        if (!min_last) low = fmaxf(low, value_of(min_key));
+      }
+      if (lane == 0) {
+        sh.limits[0] = low;
+        sh.min_key = min_key;
+      }
     }
-    // e_i >= min_p from this logit on. With both top-k and top-p S1's whole mass is needed, and the limit comes last.
-    if (s.min_p > 0.) {
-      min_key = first_key(key_of(low), [&](uint32_t key) { return weight_of(value_of(key), m, s.c) >= s.min_p; });
-      if (!min_last) low = fmaxf(low, value_of(min_key));
+    __syncthreads();  // (and the bins are clear)
+    if (s.min_p > 0. || (use_p && !use_k)) {
+      low = sh.limits[0];
+      min_key = sh.min_key;
     }
     if (use_k && s.top_k <= (int64_t)a.segs * SUBS) {
       // top_k maxima of disjoint parts of the row are that many logits: the top_k-th largest of the row is no lower than
@@ -679,7 +693,6 @@ struct Cut : Row<E, THREADS, SEGS> {
       // that is further down; the lower end of the top_k-th's will do.
       const float* subs = a.sub_max + (int64_t)r * a.segs * SUBS;
       const int n = a.segs * SUBS;
-      __syncthreads();  // (the bins are clear)
       for (int i = tid; i < n; i += THREADS) atomicAdd(&sh.step_count[min((top_key - key_of(subs[i])) >> 17, STEPS - 1u)], 1u);
       __syncthreads();
       constexpr int MINE = STEPS / THREADS;
@@ -807,8 +820,8 @@ struct Cut : Row<E, THREADS, SEGS> {
       bits = shift;
     } while (bits > LOW);
     cut_key = whole_key(prefix);
-    take = (int)want;
-    tied_out = (unsigned long long)(ties - take) * fixed_mass(cut_key);
+    take = want < ties ? (int)want : NO_INDEX;  // (where all are in, their places need not be known)
+    tied_out = (unsigned long long)(ties - want) * fixed_mass(cut_key);
   }
   // The key at which the candidates' mass reaches `least` (with top-k: top_p of S1's), within S1; the bins are clear.
   DEVI void select_mass(double least) {
@@ -842,6 +855,7 @@ struct Cut : Row<E, THREADS, SEGS> {
             if (open && cum + n4[i] >= want) {
               sh.bin = 255 - 4 * lane - i;
               sh.above = want - cum;
+              sh.bin_mass = n4[i];
               open = false;
             }
             cum += n4[i];
@@ -859,7 +873,8 @@ struct Cut : Row<E, THREADS, SEGS> {
     } while (bits > LOW);
     const uint32_t key = whole_key(prefix);
     const unsigned long long w = fixed_mass(key);
-    const int ties = w == 0 ? NO_INDEX : (int)min((want + w - 1) / w, (unsigned long long)NO_INDEX);
+    // (the last bin holds the ties; as of top-k, where all are in, their places need not be known)
+    const int ties = w == 0 || want > sh.bin_mass - w ? NO_INDEX : (int)((want + w - 1) / w);
     take = key == cut_key ? min(take, ties) : ties;
     cut_key = key;
   }
@@ -1163,19 +1178,34 @@ struct Cut : Row<E, THREADS, SEGS> {
     load_masses(mass, own);
     const double front = sh.row.scan.exclusive(own, z), target = u * z;
     const int chosen = Base::choose(begin_active, mass, front, target);
-    if (wave == 0) {
-      const int base = base_of(chosen);
-      float x[SEG_LANE];
-      double w[SEG_LANE];
-      load_seg<E>(x_row, base, a.V, lane, x);
-#pragma unroll
-      for (int j = 0; j < SEG_LANE; ++j) {
-        const double e = kept_weight(x[j], key_of(x[j]), base + place_of<E>(j, lane));
-        w[j] = x[j] >= low ? e : 0.;
-      }
-      const int token = wave_pick<E>(w, base, sh.row.target, target, lane);
-      finish_cut(token, z);
+    // One or two logits a thread: 6,400 clocks, by one wave 10,700.
+    if (tid == 0) {
+      sh.row.first = NO_INDEX;
+      sh.row.last = -1;
     }
+    constexpr int MINE = SEG / THREADS;
+    const int at = base_of(chosen) + tid * MINE;
+    double w[MINE], w_own = 0., w_all;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const float x = at + i < a.V ? E::one(x_row[min(at + i, a.V - 1)]) : neg_inf();
+      const double e = kept_weight(x, key_of(x), at + i);
+      w_own += w[i] = x >= low ? e : 0.;
+    }
+    double cum = sh.row.target + sh.row.scan.exclusive(w_own, w_all);  // (a barrier in front of the atomics)
+    int first = NO_INDEX, last = -1;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      cum += w[i];
+      if (w[i] > 0.) {
+        if (first == NO_INDEX && cum > target) first = at + i;
+        last = at + i;
+      }
+    }
+    lowest_of(first, &sh.row.first);
+    highest_of(last, &sh.row.last);
+    __syncthreads();
+    if (wave == 0) finish_cut(sh.row.first != NO_INDEX ? sh.row.first : sh.row.last, z);
   }
 };
 
