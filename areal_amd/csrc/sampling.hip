@@ -21,11 +21,11 @@ constexpr int SUBS = 16;             // maxima kept of a segment where top-k ask
 constexpr int MAX_SEGS = 4096;       // vocabularies up to 4 Mi
 constexpr int FEW_SEGS = 512;        // up to 512 Ki
 constexpr unsigned MANY_SEGS = 16384;  // from here a wave takes four segments of the first pass
-// Up to here a row has 1024 threads, beyond 512, two workgroups a CU: with top-p 0.9 400 x 151936 bf16 212 and 184 us.
+// Up to here a row has 1024 threads, beyond 512, two workgroups a CU: with top-p 0.9 400 x 151936 bf16 174 and 156 us.
 constexpr int64_t FEW_ROWS = 256;
 // Up to so many rows of at least so many segments the ones with many candidates are spread over workgroups: with top-p 0.9
-// 1 x 151936 bf16 takes 52 us spread and 80 by one workgroup, 64 rows 80 and 91, 128 rows 106 and 101; 8 x 50257 51 and 52,
-// 8 x 32000 60 and 42.
+// 1 x 151936 bf16 takes 41 us spread and 60 by one workgroup, 64 rows 67 and 79, 128 rows 92 and 87; 8 x 50257 42 and 40,
+// 8 x 32000 50 and 33.
 constexpr int64_t SPREAD_ROWS = 64, SPREAD_SEGS = 80;
 constexpr int LIST = 4096;           // candidates held in LDS
 constexpr double LOG2E = 1.4426950408889634;
