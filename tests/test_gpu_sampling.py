@@ -204,6 +204,33 @@ def test_a_row_does_not_depend_on_the_others(dev, settings):
             assert torch.equal(a[i:i + 1], b)
 
 
+@pytest.mark.parametrize("settings", [dict(top_p=0.9), dict(top_p=0.98, temperature=1.5), dict(top_k=30000), dict(min_p=0.2)],
+                         ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_rows_in_calls_of_any_size(dev, dtype, settings):
+    """Sets of thousands of logits, few of a segment's or nearly all of them, by one row's workgroup of either size or by several."""
+    g = torch.Generator(device=dev).manual_seed(15)
+    n, v = 300, 100277
+    x = torch.randn(n, v, generator=g, device=dev) * 1.8
+    x[1::4] = torch.rand(len(x[1::4]), v, generator=g, device=dev) * 0.5
+    part = torch.arange(v, device=dev) // 700
+    x[2::4] = torch.where(part % 3 == 0, x[1::4], x[2::4] - 6.0)   # segments of one kind and the other
+    x[3::4] = x[3::4].sort(1).values                                 # rising
+    x[7] = (x[7] * 4).round() / 4                                    # thousands of ties
+    x = x.to(dtype)
+    u = torch.rand(n, generator=g, device=dev)
+    whole = sample_tokens(x, u, return_kept=True, **settings)
+    for lo, hi in ((0, 1), (1, 2), (2, 3), (7, 8), (0, 20), (100, 200)):
+        got = sample_tokens(x[lo:hi], u[lo:hi], return_kept=True, **settings)
+        assert torch.equal(got.tokens, whole.tokens[lo:hi]) and torch.equal(got.kept, whole.kept[lo:hi])
+        # sums of masses in another order: 2^-24 and an error of 1e-11 each
+        torch.testing.assert_close(got.logprobs, whole.logprobs[lo:hi], rtol=2.0**-23 * 1.001, atol=4e-11)
+    rows = [0, 1, 2, 3, 7]
+    check(dev, x[rows].cpu(), u[rows].cpu(), settings)
+    got = sample_tokens(x, u, return_kept=True, **settings)
+    assert torch.equal(got.tokens, whole.tokens) and torch.equal(got.kept, whole.kept)
+
+
 def test_full_logprobs_are_the_trainers(dev):
     """What the trainer computes for the drawn tokens: fp32 sums of exponents up to ~30 binades (2^-24 each)."""
     g = torch.Generator(device=dev).manual_seed(13)
