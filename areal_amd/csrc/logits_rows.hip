@@ -380,12 +380,9 @@ struct KeptRaw {
       for (int k = 0; k < KEPT_UNIT / Elem<T>::VEC; ++k) v[i][k] = ((const typename Elem<T>::Vec*)from)[k];
     }
   }
-  DEVI void widen(float (&z)[KEPT_STEPS][KEPT_UNIT]) const {
+  DEVI void widen(int i, float* z) const {
 #pragma unroll
-    for (int i = 0; i < KEPT_STEPS; ++i) {
-#pragma unroll
-      for (int k = 0; k < KEPT_UNIT / Elem<T>::VEC; ++k) Elem<T>::widen(v[i][k], z[i] + k * Elem<T>::VEC);
-    }
+    for (int k = 0; k < KEPT_UNIT / Elem<T>::VEC; ++k) Elem<T>::widen(v[i][k], z + k * Elem<T>::VEC);
   }
 };
 // The same for the last tokens of a row.
@@ -434,17 +431,15 @@ DEVI KeptOnline kept_merge_block(KeptOnline st, KeptOnline* smem, float c2) {
   return r;
 }
 
-// Adds the logits of a lane's units whose bits are set. ALL: all are.
-template <bool ALL>
-DEVI void online_add_kept(KeptOnline& st, float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], float c2) {
+// Adds a lane's N logits, or (not ALL) those whose bit is set.
+template <bool ALL, int N>
+DEVI void online_add_kept(KeptOnline& st, float (&z)[N], uint32_t bits, float c2) {
   float xm = neg_inf();
 #pragma unroll
-  for (int k = 0; k < KEPT_STEPS; ++k)
-#pragma unroll
-    for (int i = 0; i < KEPT_UNIT; ++i) {
-      if (!ALL) z[k][i] = b[k] >> i & 1 ? z[k][i] : neg_inf();
-      xm = fmaxf(xm, z[k][i]);
-    }
+  for (int i = 0; i < N; ++i) {
+    if (!ALL) z[i] = bits >> i & 1 ? z[i] : neg_inf();
+    xm = fmaxf(xm, z[i]);
+  }
   if (xm > st.m) {
     if (st.m > neg_inf()) {
       const float d = stat_max((st.m - xm) * c2, KEPT_LOWEST), al = fast_exp2(d);
@@ -455,21 +450,17 @@ DEVI void online_add_kept(KeptOnline& st, float (&z)[KEPT_STEPS][KEPT_UNIT], con
   }
   const float m = st.m > neg_inf() ? st.m : 0.f;
 #pragma unroll
-  for (int k = 0; k < KEPT_STEPS; ++k) {
-    if (!ALL && __builtin_amdgcn_ballot_w64(b[k] != 0) == 0) continue;
-#pragma unroll
-    for (int i = 0; i < KEPT_UNIT; ++i) {
-      const float t = stat_max((z[k][i] - m) * c2, KEPT_LOWEST);
-      const float e = fast_exp2(t);
-      st.s += e;
-      st.q = fmaf(t, e, st.q);
-    }
+  for (int i = 0; i < N; ++i) {
+    const float t = stat_max((z[i] - m) * c2, KEPT_LOWEST);
+    const float e = fast_exp2(t);
+    st.s += e;
+    st.q = fmaf(t, e, st.q);
   }
 }
 
-// Bound by the latency of its scattered reads: 2048 x 151936 bf16, a quarter of the rows kept whole, reads 230 MB in 83 us
-// with blocks of 256 threads, 90 with 512, 116 with 1024 (99 without the next step's loads under way, 114 with one wait
-// per load); 93 x 50257 fp32 11.0, 8.4 and 11.4 us.
+// Bound by the latency of its scattered reads: 2048 x 151936 bf16, a quarter of the rows kept whole, reads 230 MB in 84 us
+// with blocks of 256 threads (512: 5 more, 1024: 30 more; 16 more without the next step's loads under way, 30 with one wait
+// per load); 93 x 50257 fp32 11.1, 8.8 and 10.8 us.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__ logits, int64_t ld,
                                                            const int64_t* __restrict__ labels,
@@ -484,9 +475,23 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float c2 = inv_temp * LOG2E_F;
   KeptOnline st{neg_inf(), 0.f, 0.f};
-  auto add = [&](float (&z)[KEPT_STEPS][KEPT_UNIT], const uint32_t (&b)[KEPT_STEPS], uint32_t word) {
-    if (__builtin_amdgcn_ballot_w64(word == 0xffffffffu) == ~0ull) online_add_kept<true>(st, z, b, c2);
-    else if (__builtin_amdgcn_ballot_w64(word != 0) != 0) online_add_kept<false>(st, z, b, c2);
+  // get(i, z): the logits of unit i. In a row that keeps few most of the wave's units are empty, and nothing is computed of them
+  // (2048 x 151936 bf16, a bit in one of 50 words: 52 us, 68 with all four looked at).
+  auto add = [&](auto get, const uint32_t (&b)[KEPT_STEPS], uint32_t word) {
+    if (__builtin_amdgcn_ballot_w64(word == 0xffffffffu) == ~0ull) {
+      float z[KEPT_STEPS * KEPT_UNIT];
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i) get(i, z + i * KEPT_UNIT);
+      online_add_kept<true>(st, z, 0, c2);
+    } else if (__builtin_amdgcn_ballot_w64(word != 0) != 0) {
+#pragma unroll
+      for (int i = 0; i < KEPT_STEPS; ++i) {
+        if (__builtin_amdgcn_ballot_w64(b[i] != 0) == 0) continue;
+        float z[KEPT_UNIT];
+        get(i, z);
+        online_add_kept<false>(st, z, b[i], c2);
+      }
+    }
   };
   const int whole = V / KEPT_STEP;  // steps without the row's end; a wave takes every WAVES-th
   for (int s0 = wave; s0 < whole; s0 += AHEAD * WAVES) {
@@ -503,9 +508,7 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       if (a + 1 < AHEAD) raw[(a + 1) & 1].load(x, step[a + 1] * KEPT_STEP, words[a + 1], lane);
-      float z[KEPT_STEPS][KEPT_UNIT];
-      raw[a & 1].widen(z);
-      add(z, raw[a & 1].b, words[a]);
+      add([&](int i, float* z) { raw[a & 1].widen(i, z); }, raw[a & 1].b, words[a]);
     }
   }
   if (whole * KEPT_STEP < V && wave == whole % WAVES) {
@@ -514,7 +517,10 @@ __global__ __launch_bounds__(THREADS) void kept_fwd_kernel(const T* __restrict__
     float z[KEPT_STEPS][KEPT_UNIT];
     uint32_t b[KEPT_STEPS];
     load_kept_end<T>(x, c, V, word, lane, b, z);
-    add(z, b, word);
+    add([&](int i, float* to) {
+#pragma unroll
+      for (int j = 0; j < KEPT_UNIT; ++j) to[j] = z[i][j];
+    }, b, word);
   }
   const KeptOnline r = kept_merge_block<WAVES>(st, smem, c2);
   if (threadIdx.x == 0) {
@@ -584,9 +590,11 @@ __global__ __launch_bounds__(64 * KEPT_BWD_WAVES) void kept_bwd_kernel(
     if (c + KEPT_STEP <= V) {
       KeptRaw<T> raw;
       raw.load(x, c, word, lane);
-      raw.widen(z);
 #pragma unroll
-      for (int i = 0; i < KEPT_STEPS; ++i) b[i] = raw.b[i];
+      for (int i = 0; i < KEPT_STEPS; ++i) {
+        raw.widen(i, z[i]);
+        b[i] = raw.b[i];
+      }
     } else {
       load_kept_end<T>(x, c, V, word, lane, b, z);
     }
